@@ -24,6 +24,7 @@ LIBS = {
     "libflagrot_kernels.so": ["fr_capi.cu", "fr_writer.cu", "fr_decode.cu", "fr_dequant.cu", "fr_xchg.cu"],
     "libflagrot_kivi.so": ["kv_capi.cu"],
     "libflagrot_mq.so": ["mq_capi.cu"],
+    "libflagrot_kv16.so": ["k16_capi.cu", "k16_write.cu", "k16_decode.cu", "k16_prefill.cu", "k16_evict.cu"],
     # test-only: known-answer kernels for the tcgen05 primitives of csrc/fr_tc5.cuh (not part of any C ABI)
     "libflagrot_tc5test.so": ["fr_tc5_selftest.cu"],
 }
