@@ -1,106 +1,491 @@
-// Decode attention over the 16-bit cache: one new token per row.
+// Decode attention over the 16-bit cache: one new token per row, keys and values streamed from the pages once.
+//
+//   s_j = qscale q . k_j,   p_j = 2^(s_j - ref),   o = sum_j p_j v_j / sum_j p_j
+//
+// HBM bound: a (key, kv head) costs 4 D bytes and 4 D G flops, so the kernel is a stream through shared memory with the
+// products on mma.sync (m16n8k16): the contraction has at most 8 to 32 query rows, a small share of what the tensor pipe
+// does in the time the bytes take, and its operands come straight out of the swizzled tiles with ldmatrix.
+//
+// Work: the visible keys of a (row, kv head, group of up to 32 q heads) are a segment of 32-key blocks; the segments of all
+// rows, each rounded up to four blocks, form one list which is cut into equal contiguous ranges, one per CTA.  So uneven
+// lengths need no host plan (the lengths may change under a captured graph), one long row fills the card, and many short
+// rows are not split.  A range's pieces of segments are joined through the workspace by the last CTA to arrive (in the order
+// of the pieces: the result does not depend on which one that is).
+//
+// CTA: four consumer warps and a producer warp that fills a ring of 16 KB stages (one block: 32 keys and their values) with
+// two tensor copies each; two CTAs per SM, so that a CTA's start and joins are covered by the other's stream.  NT = 1 | 2 | 4
+// tiles of 8 q heads: a block goes to one, two or all four warps.  A consumer's MMA has 16 query rows; 8 are q heads and the
+// other 8 carry, in the second product, the rounding errors of the weights: p = hi + lo, both of the cache's type, at no
+// extra cost, so a weight meets the values with an error of 2^-17 instead of 2^-9.
 #include "k16_kernels.h"
+#include "k16_tma.cuh"
 
 namespace k16 {
 namespace {
 
-// One CTA of four warps per (row, q head): warp w takes visible keys w, w + 4, ...; a lane holds D / 32 dims.  Running maximum
-// and sum per warp, joined through shared memory.
-template <int DT, int D>
-__global__ void __launch_bounds__(128) k_decode(AttnArgs a, float* scores, float* lse) {
-  constexpr int N = D / 64;          // 32-bit words (pairs of dims) per lane
-  const int Hq = a.c.Hkv * a.G, b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / a.G;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = a.c.len(b);
-  const Span sp(len - 1, a.window, a.sinks);
-  const uint32_t* qr = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + b * a.q_bs + hq * D) + lane * N;
-  float2 q[N], o[N];
-  for (int i = 0; i < N; ++i) {
-    q[i] = Elem<DT>::f2(qr[i]);
-    o[i] = make_float2(0.f, 0.f);
+constexpr int NW = 4, THREADS = 32 * (NW + 1);
+constexpr int BLK = 32;                  // keys per block
+constexpr int MAX_CTAS = 2 * 148;        // partial slots of the workspace: two per CTA
+constexpr int MAX_GT = 32;               // q heads per segment
+constexpr float LAZY = 8.f;              // the softmax reference moves when a score exceeds it by more than this (log2)
+
+__device__ int g_status;
+
+template <int D> struct Smem {
+  // a multiple of NW: a stage always goes to the same warps, whose waits on its barrier then follow its phases one by one
+  // (copies of different stages may land in any order, and a parity wait cannot tell a phase from the one two before)
+  static constexpr int STAGES = D == 128 ? 4 : 8;
+  static constexpr int STAGE = BLK * D * 4;                    // keys, values
+  static constexpr int MERGE = STAGES * STAGE;                 // float [NW][8][D]
+  static constexpr int ML = MERGE + NW * 8 * D * 4;            // float2 [NW][8]
+  static constexpr int BAR = ML + NW * 8 * 8;                  // full[STAGES], empty[STAGES]
+  static constexpr int RED = BAR + 2 * STAGES * 8;             // long long [NW + 1]; abort flag; last-arriver flag
+  static constexpr int TOTAL = RED + 64 + 1024;                // slack: the ring starts on a 1024-byte boundary
+};
+
+// a row's visible keys as blocks: [0, nsb) cover the sinks, the others start at block wb
+struct Row {
+  int len, s1, lo, nsb, wb, nblk, nv;
+  FR_DEVI void set(int len_, int window, int sinks) {
+    len = len_;
+    const Span sp(len - 1, window, sinks);
+    s1 = sp.s1;
+    lo = sp.lo;
+    wb = lo / BLK;
+    nsb = min((s1 + BLK - 1) / BLK, wb);
+    nblk = len > 0 ? nsb + (len + BLK - 1) / BLK - wb : 0;
+    nv = (nblk + 3) & ~3;
   }
-  const long long max_len = static_cast<long long>(a.c.bt_width) << a.c.page_sh;
-  float m = -INFINITY, l = 0.f;
-  const int nvis = sp.s1 + len - sp.lo;
-  for (int i = w; i < nvis; i += 4) {
-    const int j = i < sp.s1 ? i : i - sp.s1 + sp.lo;
-    const int pg = a.c.page_of(b, j), off = j & (a.c.page() - 1);
-    float s = 0.f;
-    const uint32_t* kr = reinterpret_cast<const uint32_t*>(a.c.pool + row_at(pg, a.c.Hkv, h, 0, a.c.page_sh, off, D)) + lane * N;
-    const uint32_t* vr = reinterpret_cast<const uint32_t*>(a.c.pool + row_at(pg, a.c.Hkv, h, 1, a.c.page_sh, off, D)) + lane * N;
-    for (int e = 0; e < N; ++e) {
-      const float2 k = pg >= 0 ? Elem<DT>::f2(kr[e]) : make_float2(0.f, 0.f);
-      s = fmaf(q[e].x, k.x, fmaf(q[e].y, k.y, s));
+  FR_DEVI int block(int k) const { return k < nsb ? k : wb + k - nsb; }
+  FR_DEVI bool visible(int j) const { return j < len && (j < s1 || j >= lo); }
+  FR_DEVI bool any(int j0, int j1) const { return j0 < s1 || max(j0, lo) < min(j1, len); }
+  FR_DEVI bool whole(int blk) const { return (blk + 1) * BLK <= len && (blk * BLK >= lo || (blk + 1) * BLK <= s1); }
+};
+
+// the pieces of a CTA's range, in order; every warp walks them for itself
+struct Walk {
+  const AttnArgs& a;
+  int Hv, b;
+  long long f, fend, row0, quota;
+  Row r;
+  int seg, k0, k1;                       // piece: blocks [k0, k1) of segment seg (kv head, head group) of row b
+  long long f0;                          // where the segment begins
+  FR_DEVI Walk(const AttnArgs& a_, int Hv_, long long quota_, long long begin, long long total) : a(a_), Hv(Hv_), quota(quota_) {
+    f = begin;
+    fend = min(begin + quota, total);
+    row0 = 0;
+    b = 0;
+    if (f >= fend) return;
+    const int lane = threadIdx.x & 31;
+    for (int r0 = 0;; r0 += 32) {        // the row that holds f: 32 rows at a time
+      long long n = 0;
+      if (r0 + lane < a.B) {
+        Row x;
+        x.set(a.c.len(r0 + lane), a.window, a.sinks);
+        n = static_cast<long long>(x.nv) * Hv;
+      }
+      long long s = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(~0u, s, d);
+        if (lane >= d) s += y;
+      }
+      const unsigned hit = __ballot_sync(~0u, row0 + s > f);
+      if (hit) {
+        const int w = __ffs(hit) - 1;
+        b = r0 + w;
+        row0 += __shfl_sync(~0u, s - n, w);
+        break;
+      }
+      row0 += __shfl_sync(~0u, s, 31);
     }
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    s *= a.qscale;
-    if (scores && lane == 0) scores[(static_cast<long long>(b) * Hq + hq) * max_len + j] = s;
-    const float mn = fmaxf(m, s), c = ex2(m - mn), p = ex2(s - mn);
-    m = mn;
-    l = fmaf(l, c, p);
-    for (int e = 0; e < N; ++e) {
-      const float2 v = pg >= 0 ? Elem<DT>::f2(vr[e]) : make_float2(0.f, 0.f);
-      o[e].x = fmaf(p, v.x, o[e].x * c);
-      o[e].y = fmaf(p, v.y, o[e].y * c);
-    }
+    r.set(a.c.len(b), a.window, a.sinks);
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) sm[w] = m, sl[w] = l;
-  for (int e = 0; e < N; ++e) so[w][(lane * N + e) * 2] = o[e].x, so[w][(lane * N + e) * 2 + 1] = o[e].y;
+  FR_DEVI bool next() {
+    while (f < fend) {
+      while (f - row0 >= static_cast<long long>(r.nv) * Hv) {
+        row0 += static_cast<long long>(r.nv) * Hv;
+        r.set(a.c.len(++b), a.window, a.sinks);
+      }
+      const long long off = f - row0;
+      seg = static_cast<int>(off / r.nv);
+      k0 = static_cast<int>(off - static_cast<long long>(seg) * r.nv);
+      f0 = f - k0;
+      const int n = static_cast<int>(min(static_cast<long long>(r.nv - k0), fend - f));
+      f += n;
+      k1 = min(k0 + n, r.nblk);
+      if (k1 > k0) return true;
+    }
+    return false;
+  }
+  FR_DEVI int first_cta() const { return static_cast<int>(f0 / quota); }
+  FR_DEVI int last_cta() const { return static_cast<int>((f0 + r.nblk - 1) / quota); }
+};
+
+FR_DEVI void ldsm4(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
+}
+FR_DEVI void ldsm4t(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
+}
+template <int DT> FR_DEVI void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (DT == 0)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+FR_DEVI void bar_consumers() { asm volatile("bar.sync 1, %0;\n" ::"n"(32 * NW) : "memory"); }
+
+// a bounded wait of a whole warp; one that runs out records its line, after which every wait of the CTA returns at once
+FR_DEVI void wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort, int line) {
+  if (!*abort && !tc5::mbar_wait_abortable(bar, parity, abort)) atomicCAS(&g_status, 0, line);
+  __syncwarp();
+}
+#define k16_wait(bar, parity, abort) wait_at(bar, parity, abort, __LINE__)
+
+template <int DT, int D, int NT>
+__global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map, int nhg,
+                                                       float* part, float* lse, float* scores, long long score_ld) {
+  using S = Smem<D>;
+  constexpr int STAGES = S::STAGES, KS = D / 16, ND = D / 8;                       // k steps of q . k, dim tiles of p . v
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+  const uint32_t sm = (raw + 1023) & ~1023u;
+  unsigned char* base = smem_raw + (sm - raw);
+  const uint32_t full = sm + S::BAR, empty = full + 8 * STAGES;
+  long long* red = reinterpret_cast<long long*>(base + S::RED);
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(base + S::RED + 48);
+  volatile uint32_t* flag = abort + 1;
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int Hv = a.c.Hkv * nhg, Hq = a.c.Hkv * a.G;
+  const int GT = min(a.G, MAX_GT);                             // q heads of a workspace slot
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc5::mbar_init(full + 8 * i, 1);
+      tc5::mbar_init(empty + 8 * i, NT);
+    }
+    tc5::mbar_init_fence();
+    *abort = 0;
+    tma_prefetch_map(&map);
+  }
+  // the list's length; rows that see nothing are written as zeros here
+  long long total = 0;
+  for (int b = tid; b < a.B; b += THREADS) {
+    Row r;
+    r.set(a.c.len(b), a.window, a.sinks);
+    total += static_cast<long long>(r.nv) * Hv;
+  }
+  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+  if (lane == 0) red[w] = total;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (a.c.len(b) == 0)
+      for (int i = tid; i < Hq * D / 2; i += THREADS)
+        reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + b * a.o_bs)[i] = 0;
   __syncthreads();
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float f[4], L = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    f[i] = sl[i] > 0.f ? ex2(sm[i] - M) : 0.f;
-    L += sl[i] * f[i];
+  total = 0;
+#pragma unroll
+  for (int i = 0; i <= NW; ++i) total += red[i];
+  const long long quota = max(((total + gridDim.x - 1) / gridDim.x + 3) & ~3ll, 4ll);
+  Walk wk(a, Hv, quota, static_cast<long long>(blockIdx.x) * quota, total);
+
+  // where a block's 16-key half, dim half and values are in a stage: pages of 16 tokens come as [dim half][16 keys | 16 values]
+  // per page, larger ones as [dim half][32 keys] and the same of values
+  const bool p16 = a.c.page_sh == 4;
+  const uint32_t a16 = p16 ? BLK * D * 2 : 2048u, ahalf = 4096u, av = p16 ? 2048u : BLK * D * 2;
+
+  if (w == NW) {                                               // ------------------------------------------- producer
+    const int rows_all = static_cast<int>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh);
+    int n = 0;                                                 // blocks issued
+    while (wk.next()) {
+      const int h = wk.seg / nhg;
+      const int* bt = a.c.bt + wk.b * a.c.bt_stride;
+      for (int kb = wk.k0; kb < wk.k1; kb += 32) {
+        // lane i: the pool rows of block kb + i
+        int y0 = rows_all, y1 = rows_all;
+        bool v0 = false, v1 = false;
+        if (kb + lane < wk.k1) {
+          const int blk = wk.r.block(kb + lane), j = blk * BLK;
+          if (p16) {
+            const int p = 2 * blk;
+            v0 = wk.r.any(j, j + 16);                          // a page without a visible key is not fetched
+            v1 = wk.r.any(j + 16, j + 32);
+            if (v0) {
+              const int pg = bt[p];
+              if (pg >= 0 && pg < a.c.num_pages) y0 = (pg * a.c.Hkv + h) * 32;
+            }
+            if (v1) {
+              const int pg = bt[p + 1];
+              if (pg >= 0 && pg < a.c.num_pages) y1 = (pg * a.c.Hkv + h) * 32;
+            }
+          } else {
+            v0 = v1 = true;
+            const int pg = bt[j >> a.c.page_sh];
+            if (pg >= 0 && pg < a.c.num_pages) {
+              y0 = (((pg * a.c.Hkv + h) * 2) << a.c.page_sh) + (j & (a.c.page() - 1));
+              y1 = y0 + a.c.page();
+            }
+          }
+        }
+        const int cnt = min(32, wk.k1 - kb);
+        for (int i = 0; i < cnt; ++i, ++n) {
+          const int st = n % STAGES;
+          const int r0 = __shfl_sync(~0u, y0, i), r1 = __shfl_sync(~0u, y1, i);
+          const int n0 = __shfl_sync(~0u, static_cast<int>(v0), i), n1 = __shfl_sync(~0u, static_cast<int>(v1), i);
+          if (n >= STAGES) k16_wait(empty + 8 * st, (n / STAGES - 1) & 1, abort);
+          if (lane == 0 && !*abort) {
+            const uint32_t dst = sm + st * S::STAGE;
+            tc5::mbar_expect(full + 8 * st, (n0 + n1) * (BLK * D * 2));
+            if (n0) tma3(dst, &map, 0, r0, 0, full + 8 * st);
+            if (n1) tma3(dst + BLK * D * 2, &map, 0, r1, 0, full + 8 * st);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (*abort && lane == 0)                                   // copies in flight end before the CTA does
+      for (int i = max(0, n - STAGES); i < n; ++i) tc5::mbar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1);
+    return;
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  if (threadIdx.x < D / 2) {
-    const int d = 2 * threadIdx.x;
-    float x = 0.f, y = 0.f;
-    for (int i = 0; i < 4; ++i) x = fmaf(f[i], so[i][d], x), y = fmaf(f[i], so[i][d + 1], y);
-    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + b * a.o_bs + hq * D)[threadIdx.x] = Elem<DT>::pack(x * inv, y * inv);
+
+  // -------------------------------------------------------------------------------------------------------- consumers
+  constexpr int GROUPS = NW / NT;                              // blocks worked on at once
+  const int tile = w / GROUPS, grp = w % GROUPS;
+  const int g = lane >> 2, t = lane & 3, l8 = lane & 7, lm = lane >> 3;
+  const uint32_t kx = l8 * 128 + ((lm ^ l8) << 4);             // K: matrix lm = 16-byte piece, row l8 = key
+  const uint32_t vx = ((lm & 1) * 8 + l8) * 128 + (((lm >> 1) ^ l8) << 4);   // V: matrix = (dim piece, key half)
+  float* mo = reinterpret_cast<float*>(base + S::MERGE);
+  float2* ml = reinterpret_cast<float2*>(base + S::ML);
+  int n = 0;                                                   // blocks before this piece
+  while (wk.next()) {
+    const int h = wk.seg / nhg, hg = wk.seg - h * nhg;
+    const int heads = min(a.G - hg * MAX_GT, MAX_GT);          // q heads of the segment
+    const int hq0 = h * a.G + hg * MAX_GT;
+    const int hv = heads - tile * 8;                           // ... and of this warp's tile (may be <= 0)
+    uint32_t q[KS][2];
+    {
+      const uint32_t* qr = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + wk.b * a.q_bs + (hq0 + tile * 8 + g) * D);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        q[i][0] = g < hv ? qr[i * 8 + t] : 0u;
+        q[i][1] = g < hv ? qr[i * 8 + 4 + t] : 0u;
+      }
+    }
+    float o[ND][4], ref = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float* srow = scores && g < hv ? scores + (static_cast<long long>(wk.b) * Hq + hq0 + tile * 8 + g) * score_ld + 2 * t : nullptr;
+    const int cnt = wk.k1 - wk.k0;
+    for (int i = ((grp - n) % GROUPS + GROUPS) % GROUPS; i < cnt; i += GROUPS) {
+      const int st = (n + i) % STAGES;
+      const int blk = wk.r.block(wk.k0 + i);
+      const uint32_t kt = sm + st * S::STAGE, vt = kt + av;
+      k16_wait(full + 8 * st, ((n + i) / STAGES) & 1, abort);
+      float s[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {                     // 32 dims: pieces 4 c .. 4 c + 3
+          uint32_t kf[4];
+          ldsm4(kt + (nt >> 1) * a16 + (c >> 1) * ahalf + (nt & 1) * 1024 + (kx ^ ((c & 1) << 6)), kf);
+          mma<DT>(s[nt], q[2 * c][0], 0u, q[2 * c][1], 0u, kf[0], kf[1]);
+          mma<DT>(s[nt], q[2 * c + 1][0], 0u, q[2 * c + 1][1], 0u, kf[2], kf[3]);
+        }
+      }
+      const bool whole = wk.r.whole(blk);
+      uint32_t vm[4] = {~0u, ~0u, ~0u, ~0u};                   // values of hidden keys are zeroed: 0 * NaN is NaN
+      float mx = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        s[nt][0] *= a.qscale;
+        s[nt][1] *= a.qscale;
+        if (srow) *reinterpret_cast<float2*>(srow + blk * BLK + nt * 8) = make_float2(s[nt][0], s[nt][1]);
+        if (!whole) {
+          const int j = blk * BLK + nt * 8 + 2 * t;
+          const bool a0 = wk.r.visible(j), a1 = wk.r.visible(j + 1);
+          if (!a0) s[nt][0] = -INFINITY;
+          if (!a1) s[nt][1] = -INFINITY;
+          vm[nt] = (a0 ? 0xFFFFu : 0u) | (a1 ? 0xFFFF0000u : 0u);
+        }
+        mx = fmaxf(mx, fmaxf(s[nt][0], s[nt][1]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+      if (__any_sync(~0u, mx > ref + LAZY)) {                  // (the first block: ref = -inf)
+        const float nr = fmaxf(mx, ref), f = ex2(ref - nr);
+        ref = nr;
+        l *= f;
+#pragma unroll
+        for (int x = 0; x < ND; ++x) o[x][0] *= f, o[x][1] *= f, o[x][2] *= f, o[x][3] *= f;
+      }
+      // fp16 weights are carried times 2^6: below 2^-24 its steps are absolute
+      const float off = DT == 1 ? 6.f - ref : -ref;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        const float p0 = ex2(s[nt][0] + off), p1 = ex2(s[nt][1] + off);
+        l += p0 + p1;
+        hi[nt] = Elem<DT>::pack(p0, p1);
+        const float2 r = Elem<DT>::f2(hi[nt]);
+        lo[nt] = Elem<DT>::pack(p0 - r.x, p1 - r.y);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int c = 0; c < ND; c += 2) {                      // 16 dims: pieces c, c + 1
+          uint32_t vf[4];
+          ldsm4t(vt + ks * a16 + (c >> 3) * ahalf + (vx ^ ((c & 7) << 4)), vf);
+          if (!whole) vf[0] &= vm[2 * ks], vf[1] &= vm[2 * ks + 1], vf[2] &= vm[2 * ks], vf[3] &= vm[2 * ks + 1];
+          mma<DT>(o[c], hi[2 * ks], lo[2 * ks], hi[2 * ks + 1], lo[2 * ks + 1], vf[0], vf[1]);
+          mma<DT>(o[c + 1], hi[2 * ks], lo[2 * ks], hi[2 * ks + 1], lo[2 * ks + 1], vf[2], vf[3]);
+        }
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(empty + 8 * st);
+    }
+    n += cnt;
+    // ---- join the warps of a tile, then the CTAs of a segment
+    l += __shfl_xor_sync(~0u, l, 1);
+    l += __shfl_xor_sync(~0u, l, 2);
+    if (t == 0) ml[w * 8 + g] = make_float2(ref, l);
+    float* mw = mo + (w * 8 + g) * D + 2 * t;
+    if (g < hv)
+#pragma unroll
+      for (int x = 0; x < ND; ++x) *reinterpret_cast<float2*>(mw + x * 8) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
+    bar_consumers();
+    const int c0 = wk.first_cta(), c1 = wk.last_cta();
+    float* slot = part + (static_cast<long long>(blockIdx.x) * 2 + (wk.f0 + wk.k0 == blockIdx.x * quota ? 0 : 1)) * (GT * (D + 2));
+    for (int i = tid; i < heads * (D / 2); i += 32 * NW) {
+      const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2)), w0 = (hh >> 3) * GROUPS;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int x = 0; x < GROUPS; ++x) M = fmaxf(M, ml[(w0 + x) * 8 + (hh & 7)].x);
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < GROUPS; ++x) {
+        const float2 e = ml[(w0 + x) * 8 + (hh & 7)];
+        if (e.y == 0.f) continue;                              // this warp had no block of the piece
+        const float f = ex2(e.x - M);
+        const float2 y = *reinterpret_cast<const float2*>(mo + ((w0 + x) * 8 + (hh & 7)) * D + d);
+        L = fmaf(f, e.y, L);
+        v.x = fmaf(f, y.x, v.x);
+        v.y = fmaf(f, y.y, v.y);
+      }
+      if (c0 == c1) {
+        const float inv = 1.f / L;
+        reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + wk.b * a.o_bs + (hq0 + hh) * D)[d >> 1] = Elem<DT>::pack(v.x * inv, v.y * inv);
+        if (lse && d == 0) lse[static_cast<long long>(wk.b) * Hq + hq0 + hh] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
+      } else {
+        *reinterpret_cast<float2*>(slot + hh * D + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(slot + GT * D + 2 * hh) = make_float2(M, L);
+      }
+    }
+    if (c0 != c1) {
+      __threadfence();
+      bar_consumers();
+      const long long sg = static_cast<long long>(wk.b) * Hv + wk.seg;
+      if (tid == 0) {
+        const int old = atomicAdd(a.tickets + sg, 1);
+        *flag = old == c1 - c0;
+        if (old == c1 - c0) a.tickets[sg] = 0;
+        __threadfence();
+      }
+      bar_consumers();
+      if (*flag) {
+        for (int i = tid; i < heads * (D / 2); i += 32 * NW) {
+          const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2));
+          float M = -INFINITY, L = 0.f;
+          float2 v = make_float2(0.f, 0.f);
+          for (int c = c0; c <= c1; ++c) {
+            const float* p = part + (static_cast<long long>(c) * 2 + (c == c0 && wk.f0 != c0 * quota ? 1 : 0)) * (GT * (D + 2));
+            const float2 e = __ldcg(reinterpret_cast<const float2*>(p + GT * D + 2 * hh));
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + hh * D + d));
+            const float nm = fmaxf(M, e.x), f = ex2(M - nm), x = ex2(e.x - nm);
+            M = nm;
+            L = L * f + x * e.y;
+            v.x = v.x * f + x * y.x;
+            v.y = v.y * f + x * y.y;
+          }
+          const float inv = 1.f / L;
+          reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + wk.b * a.o_bs + (hq0 + hh) * D)[d >> 1] = Elem<DT>::pack(v.x * inv, v.y * inv);
+          if (lse && d == 0) lse[static_cast<long long>(wk.b) * Hq + hq0 + hh] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
+        }
+      }
+    }
+    bar_consumers();                                           // the merge area and the flag are free again
   }
-  if (lse && threadIdx.x == 0) lse[b * Hq + hq] = M + log2f(L);
 }
 
-// weights[b, h, j] += sum over the head group of 2^(score - lse)
-__global__ void __launch_bounds__(256) k_weights(AttnArgs a, const float* scores, const float* lse) {
-  const int b = blockIdx.y / a.c.Hkv, h = blockIdx.y % a.c.Hkv, Hq = a.c.Hkv * a.G;
-  const int len = a.c.len(b), j = blockIdx.x * 256 + threadIdx.x;
+// weights[b, h, j] += sum over the head group of 2^(score - lse), a thread per key
+__global__ void __launch_bounds__(256) k_weights(AttnArgs a, const float* scores, long long score_ld, const float* lse, int chunks) {
+  const int bh = blockIdx.x / chunks, b = bh / a.c.Hkv, h = bh - b * a.c.Hkv, Hq = a.c.Hkv * a.G;
+  const int len = a.c.len(b), j = (blockIdx.x - bh * chunks) * 256 + threadIdx.x;
   const Span sp(len - 1, a.window, a.sinks);
   if (j >= len || (j >= sp.s1 && j < sp.lo)) return;
-  const long long max_len = static_cast<long long>(a.c.bt_width) << a.c.page_sh;
   float w = 0.f;
   for (int g = 0; g < a.G; ++g) {
     const long long r = static_cast<long long>(b) * Hq + h * a.G + g;
-    w += ex2(scores[r * max_len + j] - lse[r]);
+    w += ex2(scores[r * score_ld + j] - lse[r]);
   }
   a.weights[b * a.w_bs + h * a.w_hs + j] += w;
 }
 
+long long up(long long n, long long m) { return (n + m - 1) / m * m; }
+
+template <int DT, int D, int NT>
+cudaError_t launch(const AttnArgs& a, const CUtensorMap& map, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
+                   cudaStream_t st) {
+  const auto k = k_decode<DT, D, NT>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return e;
+  k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, map, nhg, part, lse, scores, ld);
+  return cudaGetLastError();
+}
+template <int DT, int D>
+cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
+                      cudaStream_t st) {
+  if (a.G <= 8) return launch<DT, D, 1>(a, map, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 16) return launch<DT, D, 2>(a, map, grid, nhg, part, lse, scores, ld, st);
+  return launch<DT, D, 4>(a, map, grid, nhg, part, lse, scores, ld, st);
+}
+
 }  // namespace
 
+// partials of two pieces per CTA | lse [rows, Hq] | scores [rows, Hq, max_len rounded up to blocks]
+static long long part_bytes(int G, int D) { return up(2ll * MAX_CTAS * (G < MAX_GT ? G : MAX_GT) * (D + 2) * 4, 256); }
 long long attn_ws_bytes(int rows, int Hkv, int G, int D, long long max_len, int weights) {
-  return 256 + (weights ? static_cast<long long>(rows) * Hkv * G * (max_len + 1) * 4 : 0);
+  const long long r = static_cast<long long>(rows) * Hkv * G;
+  return part_bytes(G, D) + (weights ? up(r * 4, 256) + r * up(max_len, BLK) * 4 : 0);
+}
+
+int decode_status() {
+  int v = -1;
+  return cudaMemcpyFromSymbol(&v, g_status, sizeof(v)) == cudaSuccess ? v : -1;
 }
 
 cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st) {
-  const long long R = static_cast<long long>(a.B) * a.c.Hkv * a.G;
-  float* lse = a.weights ? reinterpret_cast<float*>(a.ws) : nullptr;
-  float* scores = a.weights ? lse + R : nullptr;
-  const unsigned grid = static_cast<unsigned>(R);
-  if (dtype == 0) {
-    if (a.D == 128) k_decode<0, 128><<<grid, 128, 0, st>>>(a, scores, lse);
-    else k_decode<0, 64><<<grid, 128, 0, st>>>(a, scores, lse);
-  } else {
-    if (a.D == 128) k_decode<1, 128><<<grid, 128, 0, st>>>(a, scores, lse);
-    else k_decode<1, 64><<<grid, 128, 0, st>>>(a, scores, lse);
-  }
-  if (a.weights && a.c.bt_width > 0) {
-    const unsigned nb = static_cast<unsigned>((((static_cast<long long>(a.c.bt_width) << a.c.page_sh)) + 255) / 256);
-    k_weights<<<dim3(nb, a.B * a.c.Hkv), 256, 0, st>>>(a, scores, lse);
-  }
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map;
+  e = pool_map(&map, dtype, a.c.pool, (a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh, a.D, 32);
+  if (e != cudaSuccess) return e;
+  const long long R = static_cast<long long>(a.B) * a.c.Hkv * a.G, width = static_cast<long long>(a.c.bt_width) << a.c.page_sh;
+  const long long ld = up(width, BLK);
+  float* part = reinterpret_cast<float*>(a.ws);
+  float* lse = a.weights ? reinterpret_cast<float*>(a.ws + part_bytes(a.G, a.D)) : nullptr;
+  float* scores = a.weights ? lse + up(R * 4, 256) / 4 : nullptr;
+  const int nhg = (a.G + MAX_GT - 1) / MAX_GT, grid = 2 * sms < MAX_CTAS ? 2 * sms : MAX_CTAS;
+  if (dtype == 0)
+    e = a.D == 128 ? launch_nt<0, 128>(a, map, grid, nhg, part, lse, scores, ld, st) : launch_nt<0, 64>(a, map, grid, nhg, part, lse, scores, ld, st);
+  else
+    e = a.D == 128 ? launch_nt<1, 128>(a, map, grid, nhg, part, lse, scores, ld, st) : launch_nt<1, 64>(a, map, grid, nhg, part, lse, scores, ld, st);
+  if (e != cudaSuccess || !a.weights || width == 0) return e;
+  const long long chunks = (width + 255) / 256;
+  if (chunks * a.B * a.c.Hkv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  k_weights<<<static_cast<unsigned>(chunks * a.B * a.c.Hkv), 256, 0, st>>>(a, scores, ld, lse, static_cast<int>(chunks));
   return cudaGetLastError();
 }
 

@@ -105,5 +105,3 @@ cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
 }
 
 }  // namespace k16
-
-extern "C" int k16_device_status(void) { return 0; }

@@ -54,6 +54,7 @@ cudaError_t write_rows(const uint16_t* kv, long long kv_ts, long long kv_hs, con
                        int page_sh, long long num_pages, uint16_t* pool, cudaStream_t st);
 long long attn_ws_bytes(int rows, int Hkv, int G, int D, long long max_len, int weights);
 cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st);
+int decode_status();
 long long prefill_ws_bytes(int rows, int Hkv, int G, int D, long long new_tokens);
 long long prefill_tickets(int rows, int Hkv, int G, long long new_tokens);
 cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st);

@@ -161,6 +161,19 @@ def test_attn_long_and_wide(K, lens, Hkv, G, dtype):
     assert torch.equal(again, run_attn(K, q, pool, bt, ln, qs)), "two calls on the same inputs differ"
 
 
+@pytest.mark.parametrize("lens,Hkv,G,D,dtype", [([4096] * 64, 8, 4, 128, BF), ([3000, 5000, 7] * 20, 4, 12, 64, FP), ([60000], 8, 32, 128, BF)])
+def test_attn_repeated_calls_agree_bit_for_bit(K, lens, Hkv, G, D, dtype):
+    """copies that land in another order must not change what a warp reads, nor CTAs that finish in another order the join"""
+    g = gen(8)
+    pool, bt, ln = R.make_cache(lens, Hkv, D, 16, dtype, g)
+    q = queries(len(lens), G * Hkv, D, dtype, g)
+    ws = K.Workspace(len(lens), Hkv, G, D, bt.shape[1] * 16, DEV)
+    out = [torch.empty(len(lens), G * Hkv * D, dtype=dtype, device=DEV) for _ in range(60)]
+    for o in out:
+        K.attn(q, pool, bt, ln, o, ws, 0.12)
+    assert all(torch.equal(out[0], o) for o in out[1:])
+
+
 def test_attn_extreme_scores(K):
     """scores of some thousands, of both signs; a negative scale"""
     g = gen(5)
