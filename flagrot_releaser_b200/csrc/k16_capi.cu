@@ -50,7 +50,10 @@ extern "C" {
 
 int k16_abi_version(void) { return 1; }
 const char* k16_last_error(void) { return g_err; }
-int k16_device_status(void) { return decode_status(); }
+int k16_device_status(void) {
+  const int d = decode_status();
+  return d ? d : prefill_status();
+}
 int k16_chunk_bytes(int page, int D) { return 4 * page * D; }
 
 int k16_write(const void* kv, long long kv_ts, long long kv_hs, const long long* slots, int T, int Hkv, int D, int page,

@@ -58,6 +58,7 @@ int decode_status();
 long long prefill_ws_bytes(int rows, int Hkv, int G, int D, long long new_tokens);
 long long prefill_tickets(int rows, int Hkv, int G, long long new_tokens);
 cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st);
+int prefill_status();
 cudaError_t evict(const EvictArgs& a, cudaStream_t st);
 
 }  // namespace k16

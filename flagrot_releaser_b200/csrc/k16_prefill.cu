@@ -1,59 +1,448 @@
-// Attention of many new tokens over the 16-bit cache: causal, with an optional sliding window and sink tokens.
+// Attention of many new tokens over the 16-bit cache: causal, with an optional sliding window and sink tokens, on the
+// 5th-generation tensor cores.
+//
+//   S = Q K^T,   p = 2^(qscale S - ref),   O += P V,   out = O / sum p          (running reference and sum per row)
+//
+// Tensor bound: 4 D flops per (q head, query, visible key).  A work item is a pair of 128-row query tiles of one (sequence,
+// kv head): rows are tokens times the G q heads of the group, so all heads of a group share every key and value tile that is
+// fetched.  S (128 keys at a time), P and O of both tiles live in tensor memory (512 columns: S0 S1 O0 O1, P over its own S).
+//
+// CTA (one per SM, persistent): warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread per row), warp 8 issues the
+// MMAs, warp 9 takes work items and issues the tensor copies (Q once per item, K and V tiles of 128 keys through one ring).
+// The tensor pipe alternates  P0 V(j-1), Q0 K(j), P1 V(j-1), Q1 K(j):  while one tile's softmax runs, the other's products do.
+// The softmax reference is lazy: it moves when a row's maximum has grown by more than 2^8, and only then is O rescaled.
+//
+// V is taken as it lies (keys by dims): the second product's B operand is MN-major, K = keys.
+// P is rounded to the cache's type (2^-9 relative in bf16, 2^-12 in fp16: one rounding, like the output's own); the row sums,
+// S and O are 32-bit.
 #include "k16_kernels.h"
+#include "k16_tma.cuh"
 
 namespace k16 {
 namespace {
 
-// One warp per (token, q head); a lane holds D / 32 dims; running maximum and sum.
+constexpr int BN = 128;                  // keys per block
+constexpr int THREADS = 320;
+constexpr int W_MMA = 8, W_TMA = 9;
+constexpr int MAX_HEADS = 128;           // q heads per item
+constexpr float LAZY = 8.f;
+
+__device__ int g_status;
+
+struct Item {
+  int b, h, hq0, heads;                  // sequence, kv head, first q head and their number
+  int tok0, tok1;                        // tokens of the pair
+  int pos0;                              // position of tok0
+  int len;
+  int nsb, wb, nblk;                     // key blocks: the first nsb hold the sinks, the others start at block wb
+  FR_DEVI int block(int k) const { return k < nsb ? k : wb + k - nsb; }
+};
+// the tokens of one tile, as positions [pa, pb]
+struct Tile {
+  int pa, pb, last, window, sinks;       // last: index of the last block that the tile needs (-1: none)
+  FR_DEVI Tile(const Item& it, int i, int tpt, int window_, int sinks_) : window(window_), sinks(sinks_) {
+    pa = it.pos0 + i * tpt;
+    pb = min(it.pos0 + it.tok1 - it.tok0, pa + tpt) - 1;
+    last = pb >= max(pa, 0) ? it.nsb + pb / BN - it.wb : -1;
+  }
+  FR_DEVI bool needs(int kb) const {
+    return last >= 0 && kb <= pb && (window <= 0 || kb + BN > pa - window + 1 || kb < sinks);
+  }
+  FR_DEVI bool whole(int kb) const { return kb + BN - 1 <= pa && (window <= 0 || kb > pb - window || kb + BN <= sinks); }
+};
+
+template <int D> struct Smem {
+  static constexpr int QT = 128 * D * 2;                       // one query tile
+  static constexpr int STAGE = BN * D * 2;                     // one K or V tile
+  static constexpr int STAGES = D == 128 ? 5 : 10;
+  static constexpr int RING = 2 * QT;
+  static constexpr int BAR = RING + STAGES * STAGE;            // full[STAGES] empty[STAGES] qfull qempty sfull[2] pfull[2] ofull[2]
+  static constexpr int NBAR = 2 * STAGES + 2 + 6 + 4;          // ... items: full[2], empty[2]
+  static constexpr int ITEMS = BAR + NBAR * 8;                 // Item[2]
+  static constexpr int MISC = ITEMS + 2 * 64;                  // tensor-memory base, abort flag
+  static constexpr int TOTAL = MISC + 16 + 1024;
+};
+static_assert(sizeof(Item) <= 64, "item slot");
+static_assert(Smem<128>::TOTAL <= 232448, "shared memory");
+
+FR_DEVI bool wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort, int line) {
+  bool ok = true;
+  if (!tc5::mbar_try(bar, parity)) {
+    ok = !*abort && tc5::mbar_wait_abortable(bar, parity, abort);
+    if (!ok) atomicCAS(&g_status, 0, line);
+  }
+  return __all_sync(~0u, ok);
+}
+#define k16_wait(bar, parity) wait_at(bar, parity, abort, __LINE__)
+
+// MN-major operand in 128-byte swizzle: lbo = bytes between 64-element chunks along N, sbo = bytes between groups of 8 keys
+FR_DEVI uint64_t desc_mn(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return tc5::DESC_VERSION | tc5::DESC_SW128 | (static_cast<uint64_t>(sbo >> 4) << 32) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+         ((saddr & 0x3FFFFu) >> 4);
+}
+constexpr uint32_t B_MN_MAJOR = 1u << 16;                      // instruction descriptor: B is MN-major
+
 template <int DT, int D>
-__global__ void __launch_bounds__(128) k_prefill(PrefillArgs a) {
-  constexpr int N = D / 64;
-  const int Hq = a.c.Hkv * a.G, lane = threadIdx.x & 31;
-  const long long item = blockIdx.x * 4ll + (threadIdx.x >> 5);
-  const int t = static_cast<int>(item / Hq), hq = static_cast<int>(item % Hq), h = hq / a.G;
-  if (t >= a.T) return;
-  // the sequence of token t: the last row that begins at or before it
-  int b0 = 0, b1 = a.B;              // cu_q[b0] <= t < cu_q[b1] when t belongs to any
-  while (b1 - b0 > 1) {
-    const int mid = (b0 + b1) >> 1;
-    if (a.cu_q[mid] <= t) b0 = mid; else b1 = mid;
-  }
-  const int beg = a.cu_q[b0], end = a.cu_q[b0 + 1];
-  if (t < beg || t >= end) return;
-  const int len = a.c.len(b0), pos = len - end + t;
-  const Span sp(pos, a.window, a.sinks);
-  const uint32_t* qr = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + t * a.q_ts + hq * D) + lane * N;
-  float2 q[N], o[N];
-  for (int i = 0; i < N; ++i) {
-    q[i] = Elem<DT>::f2(qr[i]);
-    o[i] = make_float2(0.f, 0.f);
-  }
-  float m = -INFINITY, l = 0.f;
-  const int nvis = pos < 0 ? 0 : sp.s1 + pos + 1 - sp.lo;
-  for (int i = 0; i < nvis; ++i) {
-    const int j = i < sp.s1 ? i : i - sp.s1 + sp.lo;
-    const int pg = a.c.page_of(b0, j), off = j & (a.c.page() - 1);
-    const uint32_t* kr = reinterpret_cast<const uint32_t*>(a.c.pool + row_at(pg, a.c.Hkv, h, 0, a.c.page_sh, off, D)) + lane * N;
-    const uint32_t* vr = reinterpret_cast<const uint32_t*>(a.c.pool + row_at(pg, a.c.Hkv, h, 1, a.c.page_sh, off, D)) + lane * N;
-    float s = 0.f;
-    for (int e = 0; e < N; ++e) {
-      const float2 k = pg >= 0 ? Elem<DT>::f2(kr[e]) : make_float2(0.f, 0.f);
-      s = fmaf(q[e].x, k.x, fmaf(q[e].y, k.y, s));
+__global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
+                                                        const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
+  using S = Smem<D>;
+  constexpr int STAGES = S::STAGES, HALVES = D / 64;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+  const uint32_t sm = (raw + 1023) & ~1023u;
+  unsigned char* base = smem_raw + (sm - raw);
+  const uint32_t full = sm + S::BAR, empty = full + 8 * STAGES, qfull = empty + 8 * STAGES, qempty = qfull + 8, sfull = qempty + 8,
+                 pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base + S::MISC);
+  volatile uint32_t* abort = tmem_slot + 1;
+  Item* items = reinterpret_cast<Item*>(base + S::ITEMS);
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc5::mbar_init(full + 8 * i, 1);
+      tc5::mbar_init(empty + 8 * i, 1);
     }
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    s *= a.qscale;
-    const float mn = fmaxf(m, s), c = ex2(m - mn), p = ex2(s - mn);
-    m = mn;
-    l = fmaf(l, c, p);
-    for (int e = 0; e < N; ++e) {
-      const float2 v = pg >= 0 ? Elem<DT>::f2(vr[e]) : make_float2(0.f, 0.f);
-      o[e].x = fmaf(p, v.x, o[e].x * c);
-      o[e].y = fmaf(p, v.y, o[e].y * c);
+    tc5::mbar_init(qfull, 1);
+    tc5::mbar_init(qempty, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(sfull + 8 * i, 1);
+      tc5::mbar_init(pfull + 8 * i, 4);
+      tc5::mbar_init(ofull + 8 * i, 1);
+      tc5::mbar_init(ifull + 8 * i, 1);
+      tc5::mbar_init(iempty + 8 * i, 9);
+    }
+    tc5::mbar_init_fence();
+    *abort = 0;
+    tma_prefetch_map(&qmap);
+    tma_prefetch_map(&kvmap);
+  }
+  if (w == W_MMA) {
+    tc5::tmem_alloc(sm + S::MISC, 512);
+    tc5::tmem_relinquish();
+  }
+  tc5::fence_before_sync();
+  __syncthreads();
+  tc5::fence_after_sync();
+  const uint32_t tm = *tmem_slot;
+  const uint32_t tS = tm, tO = tm + 256;                       // columns: S0 128 | S1 128 | O0 128 | O1 128
+  const int tpt = 128 / hb;                                    // tokens per tile; row = token * hb + head
+
+  if (w == W_TMA) {                                            // ----------------------------------- items and tensor copies
+    const int Hv = a.c.Hkv * nhg;
+    const int rows_all = static_cast<int>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh);
+    const int nbox = BN / box_rows, box_sh = __ffs(box_rows) - 1;
+    int n = 0, qc = 0;                                         // ring tiles and query pairs issued
+    // 32 sequences at a time: lane i has sequence r0 + i, its tokens, its items and the items up to and with it
+    int r0 = -32, beg = 0, end = 0;
+    long long mine = 0, upto = 0, row0 = 0, group = 0;         // row0: items before the 32
+    long long idx = blockIdx.x;
+    for (int ic = 0;; ++ic, idx += gridDim.x) {
+      Item it;
+      it.b = -1;
+      while (r0 < a.B && idx >= row0 + group) {                // (indices only grow)
+        row0 += group;
+        r0 += 32;
+        const int b = r0 + lane;
+        beg = end = 0;
+        if (b < a.B) {
+          beg = min(max(a.cu_q[b], 0), a.T);
+          end = min(max(a.cu_q[b + 1], beg), a.T);
+        }
+        mine = static_cast<long long>((end - beg + 2 * tpt - 1) / (2 * tpt)) * Hv;
+        upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const long long y = __shfl_up_sync(~0u, upto, d);
+          if (lane >= d) upto += y;
+        }
+        group = __shfl_sync(~0u, upto, 31);
+      }
+      if (r0 < a.B) {                                          // a head's pairs side by side, the longest first
+        const int src = __ffs(__ballot_sync(~0u, row0 + upto > idx)) - 1, b = r0 + src;
+        const int off = static_cast<int>(idx - row0 - __shfl_sync(~0u, upto - mine, src));
+        const int npairs = static_cast<int>(__shfl_sync(~0u, mine, src) / Hv);
+        const int sbeg = __shfl_sync(~0u, beg, src), send = __shfl_sync(~0u, end, src);
+        const int hv = off / npairs, pr = npairs - 1 - (off - hv * npairs);
+        it.b = b;
+        it.h = hv / nhg;
+        const int hg = hv - it.h * nhg;
+        it.hq0 = it.h * a.G + hg * hb;
+        it.heads = min(a.G - hg * hb, hb);
+        it.tok0 = sbeg + pr * 2 * tpt;
+        it.tok1 = min(it.tok0 + 2 * tpt, send);
+        it.len = a.c.len(b);
+        it.pos0 = it.len - send + it.tok0;
+        const int p1 = it.pos0 + it.tok1 - it.tok0 - 1;
+        const Span sp(max(it.pos0, 0), a.window, a.sinks);
+        it.wb = sp.lo / BN;
+        it.nsb = min((min(a.sinks, sp.lo) + BN - 1) / BN, it.wb);
+        it.nblk = p1 >= 0 ? it.nsb + p1 / BN - it.wb + 1 : 0;
+      }
+      const int sl = ic & 1;
+      if (ic >= 2 && !k16_wait(iempty + 8 * sl, (ic / 2 - 1) & 1)) break;
+      if (lane == 0) {
+        items[sl] = it;
+        tc5::mbar_arrive(ifull + 8 * sl);
+      }
+      __syncwarp();
+      if (it.b < 0) break;
+      if (it.nblk == 0) continue;
+      // queries: [D half][token][head] = rows of 128 bytes; what lies outside q arrives as zeros
+      if (qc > 0 && !k16_wait(qempty, (qc - 1) & 1)) break;
+      if (lane == 0) {
+        tc5::mbar_expect(qfull, 2 * HALVES * tpt * hb * 128);
+        for (int i = 0; i < 2; ++i)
+          for (int x = 0; x < HALVES; ++x)
+            tma4(sm + i * S::QT + x * 128 * 128, &qmap, 0, it.hq0, it.tok0 + i * tpt, x, qfull);
+      }
+      ++qc;
+      const int* bt = a.c.bt + it.b * a.c.bt_stride;
+      bool ok = true;
+      for (int k = 0; k < it.nblk && ok; ++k) {
+        const int j = it.block(k) * BN + lane * box_rows;      // lane i < nbox: box i of the block
+        int y = rows_all;
+        if (lane < nbox && j < it.len) {
+          const int pg = bt[j >> a.c.page_sh];
+          if (pg >= 0 && pg < a.c.num_pages)
+            y = ((pg * a.c.Hkv + it.h) * 2 << a.c.page_sh) + (j & (a.c.page() - 1));
+        }
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const int st = n % STAGES;
+          if (n >= STAGES && !k16_wait(empty + 8 * st, (n / STAGES - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) tc5::mbar_expect(full + 8 * st, S::STAGE);
+          __syncwarp();
+          if (lane < nbox) {
+            const uint32_t dst = sm + S::RING + st * S::STAGE + (lane << (box_sh + 7));
+            const int yy = y == rows_all ? y : y + (kv << a.c.page_sh);
+            for (int x = 0; x < HALVES; ++x) tma3(dst + x * BN * 128, &kvmap, 0, yy, x, full + 8 * st);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok) break;
+    }
+    // the CTA ends after its copies and its commits on the ring have arrived (bounded, also when a wait has run out)
+    for (int i = max(0, n - STAGES); i < n && lane == 0; ++i) {
+      if (!*abort && tc5::mbar_wait(empty + 8 * (i % STAGES), (i / STAGES) & 1)) continue;
+      tc5::mbar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1);
+    }
+    if (*abort && lane == 0 && qc) tc5::mbar_wait(qfull, (qc - 1) & 1);
+  } else if (w == W_MMA) {                                     // ------------------------------------------------------ MMAs
+    constexpr uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, BN);
+    constexpr uint32_t ID_PV = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, D) | B_MN_MAJOR;
+    int n = 0, qc = 0, pc[2] = {0, 0};                         // ring tiles, query pairs, P tiles consumed
+    bool run = true;
+    for (int ic = 0; run; ++ic) {
+      const int sl = ic & 1;
+      if (!k16_wait(ifull + 8 * sl, (ic / 2) & 1)) break;
+      const Item it = items[sl];
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(iempty + 8 * sl);
+      if (it.b < 0) break;
+      if (it.nblk == 0) continue;
+      const Tile t0(it, 0, tpt, a.window, a.sinks), t1(it, 1, tpt, a.window, a.sinks);
+      if (!k16_wait(qfull, qc & 1)) break;
+      ++qc;
+      tc5::fence_after_sync();
+      bool started[2] = {false, false};
+      for (int k = 0; k <= it.nblk && run; ++k) {
+        const int nv = n + 2 * k - 1, nk = n + 2 * k;          // ring tiles of V(k - 1) and K(k)
+        const uint32_t sv = sm + S::RING + (nv % STAGES) * S::STAGE, sk = sm + S::RING + (nk % STAGES) * S::STAGE;
+        const int kbv = k > 0 ? it.block(k - 1) * BN : 0, kbk = k < it.nblk ? it.block(k) * BN : 0;
+        if (k > 0) {
+          if (!(run = k16_wait(full + 8 * (nv % STAGES), (nv / STAGES) & 1))) break;
+          if (kbv + BN > it.len) {                             // values behind the sequence: 0 * NaN would be NaN
+            for (int i = (it.len - kbv) * 8 + lane; i < BN * 8; i += 32)
+#pragma unroll
+              for (int x = 0; x < HALVES; ++x)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + i * 16), "r"(0) : "memory");
+            tc5::fence_async_smem();
+            __syncwarp();
+          }
+        }
+        bool have_k = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const Tile& t = i ? t1 : t0;
+          if (k > 0 && t.needs(kbv)) {
+            if (!(run = k16_wait(pfull + 8 * i, pc[i] & 1))) break;
+            ++pc[i];
+            tc5::fence_after_sync();
+            if (tc5::elect_one()) {
+#pragma unroll
+              for (int s = 0; s < BN / 16; ++s)
+                tc5::mma_f16_ts(tO + i * 128, tS + i * 128 + s * 8, desc_mn(sv + s * 2048, BN * 128, 1024), ID_PV, started[i] || s > 0);
+              if (k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
+            }
+            __syncwarp();
+            started[i] = true;
+          }
+          if (k < it.nblk && !have_k) {
+            if (!(run = k16_wait(full + 8 * (nk % STAGES), (nk / STAGES) & 1))) break;
+            have_k = true;
+            tc5::fence_after_sync();
+          }
+          if (k < it.nblk && t.needs(kbk)) {
+            if (tc5::elect_one()) {
+#pragma unroll
+              for (int s = 0; s < D / 16; ++s)
+                tc5::mma_f16_ss(tS + i * 128, tc5::desc_sw128(sm + i * S::QT + (s >> 2) * 128 * 128 + (s & 3) * 32, 1024),
+                                tc5::desc_sw128(sk + (s >> 2) * BN * 128 + (s & 3) * 32, 1024), ID_QK, s > 0);
+              tc5::mma_commit(sfull + 8 * i);
+            }
+            __syncwarp();
+          }
+        }
+        if (!run) break;
+        if (tc5::elect_one()) {
+          if (k > 0) tc5::mma_commit(empty + 8 * (nv % STAGES));
+          if (k < it.nblk) tc5::mma_commit(empty + 8 * (nk % STAGES));
+          if (k == it.nblk - 1) tc5::mma_commit(qempty);
+        }
+        __syncwarp();
+      }
+      n += 2 * it.nblk;
+    }
+  } else {                                                     // --------------------------------------------------- softmax
+    const int i = w >> 2, r = tid & 127, tok = r / hb, head = r - tok * hb;
+    const uint32_t lanes = static_cast<uint32_t>(w & 3) << 21;  // tensor-memory lanes of this warp
+    const uint32_t ts = tS + i * 128 + lanes, to = tO + i * 128 + lanes;
+    const bool neg = a.qscale < 0.f;                           // the maximum is taken of |qscale| (+-S)
+    const float qs = fmaxf(fabsf(a.qscale), 1e-37f);           // a scale of 0: all scores alike, and -inf * qs stays -inf
+    constexpr float BIAS = DT == 1 ? 6.f : 0.f;                // fp16 weights are carried times 2^6: their steps below 2^-14 are absolute
+    int sc = 0, oc = 0;                                        // S and O tiles consumed
+    bool run = true;
+    for (int ic = 0; run; ++ic) {
+      const int sl = ic & 1;
+      if (!k16_wait(ifull + 8 * sl, (ic / 2) & 1)) break;
+      const Item it = items[sl];
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(iempty + 8 * sl);
+      if (it.b < 0) break;
+      const Tile t(it, i, tpt, a.window, a.sinks);
+      const int mytok = it.tok0 + i * tpt + tok;
+      const bool live = tok < tpt && head < it.heads && mytok < it.tok1;
+      const int pos = live ? it.pos0 + i * tpt + tok : -1;
+      float ref = -INFINITY, l = 0.f;
+      for (int k = 0; k < it.nblk; ++k) {
+        const int kb = it.block(k) * BN;
+        if (!t.needs(kb)) continue;
+        if (!(run = k16_wait(sfull + 8 * i, sc & 1))) break;
+        ++sc;
+        tc5::fence_after_sync();
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc5::tmem_ld32(ts + 32 * c, v[c]);
+        tc5::tmem_ld_wait();
+        if (neg)
+#pragma unroll
+          for (int c = 0; c < 128; ++c) v[c >> 5][c & 31] ^= 0x80000000u;
+        if (!t.whole(kb)) {
+          const int hi = pos - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : -1, sk = a.sinks - kb;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (!(c <= hi && (c >= lo || c < sk))) v[c >> 5][c & 31] = 0xFF800000u;
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          m0 = fmaxf(m0, __uint_as_float(v[0][c]));
+          m1 = fmaxf(m1, __uint_as_float(v[1][c]));
+          m2 = fmaxf(m2, __uint_as_float(v[2][c]));
+          m3 = fmaxf(m3, __uint_as_float(v[3][c]));
+        }
+        const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
+        if (__any_sync(~0u, m > ref + LAZY)) {
+          const float nr = fmaxf(m, ref), f = ref == -INFINITY ? 0.f : ex2(ref - nr);
+          // S(k) is complete, so every product into O before it is; the next one waits for this P
+          if (__any_sync(~0u, l > 0.f)) {
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tc5::tmem_ld32(to + 32 * c, o);
+              tc5::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc5::tmem_st32(to + 32 * c, o);
+            }
+          }
+          ref = nr;
+        }
+        const float off = (ref == -INFINITY ? 0.f : -ref) + BIAS;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int x = 64 * c + 2 * e;
+            const float p0 = ex2(fmaf(__uint_as_float(v[x >> 5][x & 31]), qs, off));
+            const float p1 = ex2(fmaf(__uint_as_float(v[x >> 5][(x & 31) + 1]), qs, off));
+            l0 += p0;
+            l1 += p1;
+            p[e] = Elem<DT>::pack(p0, p1);
+          }
+          tc5::tmem_st32(ts + 32 * c, p);
+        }
+        l += l0 + l1;
+        tc5::tmem_st_wait();
+        tc5::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive(pfull + 8 * i);
+      }
+      if (!run) break;
+      const bool any = t.last >= 0;
+      if (any) {
+        if (!(run = k16_wait(ofull + 8 * i, oc & 1))) break;
+        ++oc;
+        tc5::fence_after_sync();
+      }
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;     // a row that sees nothing gives zeros; NaN stays NaN
+      uint16_t* out = static_cast<uint16_t*>(a.out) + mytok * a.o_ts + (it.hq0 + head) * D;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tc5::tmem_ld32(to + 32 * c, o);
+          tc5::tmem_ld_wait();
+        }
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (any && inv != 0.f) {
+              x.x = Elem<DT>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+              x.y = Elem<DT>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              x.z = Elem<DT>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              x.w = Elem<DT>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            }
+            *reinterpret_cast<uint4*>(out + 32 * c + e) = x;
+          }
+        }
+        __syncwarp();
+      }
+      tc5::fence_before_sync();
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + t * a.o_ts + hq * D) + lane * N;
-  for (int e = 0; e < N; ++e) out[e] = Elem<DT>::pack(o[e].x * inv, o[e].y * inv);
+  tc5::fence_before_sync();
+  __syncthreads();
+  if (w == W_MMA) {
+    tc5::fence_after_sync();
+    tc5::tmem_dealloc(tm, 512);
+  }
+}
+
+template <int DT, int D>
+cudaError_t launch(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int grid, cudaStream_t st) {
+  const auto k = k_prefill<DT, D>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return e;
+  k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, qm, kv, hb, nhg, box);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -61,17 +450,29 @@ __global__ void __launch_bounds__(128) k_prefill(PrefillArgs a) {
 long long prefill_ws_bytes(int, int, int, int, long long) { return 0; }
 long long prefill_tickets(int, int, int, long long) { return 0; }
 
+int prefill_status() {
+  int v = -1;
+  return cudaMemcpyFromSymbol(&v, g_status, sizeof(v)) == cudaSuccess ? v : -1;
+}
+
 cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
-  const long long n = static_cast<long long>(a.T) * a.c.Hkv * a.G;
-  const unsigned grid = static_cast<unsigned>((n + 3) / 4);
-  if (dtype == 0) {
-    if (a.D == 128) k_prefill<0, 128><<<grid, 128, 0, st>>>(a);
-    else k_prefill<0, 64><<<grid, 128, 0, st>>>(a);
-  } else {
-    if (a.D == 128) k_prefill<1, 128><<<grid, 128, 0, st>>>(a);
-    else k_prefill<1, 64><<<grid, 128, 0, st>>>(a);
-  }
-  return cudaGetLastError();
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const int nhg = (a.G + MAX_HEADS - 1) / MAX_HEADS, hb = (a.G + nhg - 1) / nhg, tpt = 128 / hb, Hq = a.c.Hkv * a.G;
+  const int box = 1 << a.c.page_sh;                            // page <= 128 = BN rows
+  CUtensorMap qm, kv;
+  e = encode4(&qm, dtype, a.q, Hq, a.D * 2ull, a.T, a.T > 1 ? a.q_ts * 2ull : Hq * a.D * 2ull, a.D / 64, 128, hb, tpt);
+  if (e == cudaSuccess)
+    e = encode3(&kv, dtype, a.c.pool, static_cast<uint64_t>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh), a.D * 2ull, a.D / 64, 128, box, 1);
+  if (e != cudaSuccess) return e;
+  // items at most: every sequence may end inside a pair
+  const long long items = (static_cast<long long>(a.T) / (2 * tpt) + a.B) * a.c.Hkv * nhg;
+  const int grid = static_cast<int>(items < sms ? items : sms);
+  if (dtype == 0)
+    return a.D == 128 ? launch<0, 128>(a, qm, kv, hb, nhg, box, grid, st) : launch<0, 64>(a, qm, kv, hb, nhg, box, grid, st);
+  return a.D == 128 ? launch<1, 128>(a, qm, kv, hb, nhg, box, grid, st) : launch<1, 64>(a, qm, kv, hb, nhg, box, grid, st);
 }
 
 }  // namespace k16

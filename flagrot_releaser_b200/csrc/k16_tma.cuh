@@ -40,6 +40,18 @@ inline cudaError_t encode3(CUtensorMap* m, int dtype, const void* base, uint64_t
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
+// box of 64 elements x b1 x b2 x 1
+inline cudaError_t encode4(CUtensorMap* m, int dtype, const void* base, uint64_t d1, uint64_t s1, uint64_t d2, uint64_t s2, uint64_t d3,
+                           uint64_t s3, uint32_t b1, uint32_t b2) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[4] = {64, d1, d2, d3}, strides[3] = {s1, s2, s3};
+  const cuuint32_t box[4] = {64, b1, b2, 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                        dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
 inline cudaError_t pool_map(CUtensorMap* m, int dtype, const void* pool, long long rows, int D, uint32_t box_rows) {
   return encode3(m, dtype, pool, static_cast<uint64_t>(rows), static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(D / 64), 128, box_rows,
                  static_cast<uint32_t>(D / 64));
@@ -48,6 +60,11 @@ inline cudaError_t pool_map(CUtensorMap* m, int dtype, const void* pool, long lo
 FR_DEVI void tma3(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t mbar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
                "l"(m), "r"(x), "r"(y), "r"(z), "r"(mbar)
+               : "memory");
+}
+FR_DEVI void tma4(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint32_t mbar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+               "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(mbar)
                : "memory");
 }
 FR_DEVI void tma_prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(m) : "memory"); }
