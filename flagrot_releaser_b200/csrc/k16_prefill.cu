@@ -22,8 +22,9 @@ namespace k16 {
 namespace {
 
 constexpr int BN = 128;                  // keys per block
-constexpr int THREADS = 320;
+constexpr int THREADS = 384;            // three warpgroups: two of softmax, one of MMA, copies and two idle warps
 constexpr int W_MMA = 8, W_TMA = 9;
+constexpr int REGS_SOFT = 216, REGS_REST = 72;   // 256 x 216 + 128 x 72 = 384 x 168, what the launch has
 constexpr int MAX_HEADS = 128;           // q heads per item
 constexpr float LAZY = 8.f;
 
@@ -82,6 +83,35 @@ FR_DEVI uint64_t desc_mn(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
 }
 constexpr uint32_t B_MN_MAJOR = 1u << 16;                      // instruction descriptor: B is MN-major
 
+// two floats in one register pair; each half is rounded like the scalar operation
+FR_DEVI uint64_t pk(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+FR_DEVI float2 un(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+FR_DEVI uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FR_DEVI uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+FR_DEVI float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// the n lowest of 32 bits
+FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
                                                         const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
@@ -128,7 +158,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
   const uint32_t tS = tm, tO = tm + 256;                       // columns: S0 128 | S1 128 | O0 128 | O1 128
   const int tpt = 128 / hb;                                    // tokens per tile; row = token * hb + head
 
-  if (w == W_TMA) {                                            // ----------------------------------- items and tensor copies
+  if (w >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_REST));
+  if (w > W_TMA) {
+    // (idle)
+  } else if (w == W_TMA) {                                            // ----------------------------------- items and tensor copies
     const int Hv = a.c.Hkv * nhg;
     const int rows_all = static_cast<int>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh);
     const int nbox = BN / box_rows, box_sh = __ffs(box_rows) - 1;
@@ -308,6 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       n += 2 * it.nblk;
     }
   } else {                                                     // --------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFT));
     const int i = w >> 2, r = tid & 127, tok = r / hb, head = r - tok * hb;
     const uint32_t lanes = static_cast<uint32_t>(w & 3) << 21;  // tensor-memory lanes of this warp
     const uint32_t ts = tS + i * 128 + lanes, to = tO + i * 128 + lanes;
@@ -342,18 +376,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 #pragma unroll
           for (int c = 0; c < 128; ++c) v[c >> 5][c & 31] ^= 0x80000000u;
         if (!t.whole(kb)) {
-          const int hi = pos - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : -1, sk = a.sinks - kb;
+          const int hi = pos + 1 - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : 0, sk = a.sinks - kb;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (!(c <= hi && (c >= lo || c < sk))) v[c >> 5][c & 31] = 0xFF800000u;
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t see = low_bits(hi - 32 * c) & (~low_bits(lo - 32 * c) | low_bits(sk - 32 * c));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(see & (1u << e))) v[c][e] = 0xFF800000u;
+          }
         }
         float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          m0 = fmaxf(m0, __uint_as_float(v[0][c]));
-          m1 = fmaxf(m1, __uint_as_float(v[1][c]));
-          m2 = fmaxf(m2, __uint_as_float(v[2][c]));
-          m3 = fmaxf(m3, __uint_as_float(v[3][c]));
+        for (int c = 0; c < 32; c += 2) {
+          m0 = max3(m0, __uint_as_float(v[0][c]), __uint_as_float(v[0][c + 1]));
+          m1 = max3(m1, __uint_as_float(v[1][c]), __uint_as_float(v[1][c + 1]));
+          m2 = max3(m2, __uint_as_float(v[2][c]), __uint_as_float(v[2][c + 1]));
+          m3 = max3(m3, __uint_as_float(v[3][c]), __uint_as_float(v[3][c + 1]));
         }
         const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
         if (__any_sync(~0u, m > ref + LAZY)) {
@@ -374,22 +412,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           ref = nr;
         }
         const float off = (ref == -INFINITY ? 0.f : -ref) + BIAS;
-        float l0 = 0.f, l1 = 0.f;
+        const uint64_t q2 = pk(qs, qs), off2 = pk(off, off);
+        uint64_t sum = 0, sum1 = 0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t p[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int x = 64 * c + 2 * e;
-            const float p0 = ex2(fmaf(__uint_as_float(v[x >> 5][x & 31]), qs, off));
-            const float p1 = ex2(fmaf(__uint_as_float(v[x >> 5][(x & 31) + 1]), qs, off));
-            l0 += p0;
-            l1 += p1;
+            const float2 y = un(fma2(pk(__uint_as_float(v[x >> 5][x & 31]), __uint_as_float(v[x >> 5][(x & 31) + 1])), q2, off2));
+            const float p0 = ex2(y.x), p1 = ex2(y.y);
+            if (e & 1) sum1 = add2(sum1, pk(p0, p1));
+            else sum = add2(sum, pk(p0, p1));
             p[e] = Elem<DT>::pack(p0, p1);
           }
           tc5::tmem_st32(ts + 32 * c, p);
         }
-        l += l0 + l1;
+        const float2 l2 = un(add2(sum, sum1));
+        l += l2.x + l2.y;
         tc5::tmem_st_wait();
         tc5::fence_before_sync();
         __syncwarp();
