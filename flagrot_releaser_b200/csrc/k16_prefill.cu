@@ -27,6 +27,9 @@ constexpr int W_MMA = 8, W_TMA = 9;
 constexpr int REGS_SOFT = 216, REGS_REST = 72;   // 256 x 216 + 128 x 72 = 384 x 168, what the launch has
 constexpr int MAX_HEADS = 128;           // q heads per item
 constexpr float LAZY = 8.f;
+constexpr int MAX_SPLIT = 32;            // pieces of a pair's key blocks
+constexpr int SLOTS = 2 * 148;           // workspace slots: pieces of split pairs
+constexpr int SPLIT_COST = 4;            // what a piece costs besides its blocks, in blocks
 
 __device__ int g_status;
 
@@ -35,20 +38,23 @@ struct Item {
   int tok0, tok1;                        // tokens of the pair
   int pos0;                              // position of tok0
   int len;
-  int nsb, wb, nblk;                     // key blocks: the first nsb hold the sinks, the others start at block wb
+  int nsb, wb;                           // key blocks: the first nsb hold the sinks, the others start at block wb
+  int k0, k1;                            // ... of which this item takes [k0, k1)
+  int ns, part, slot, stride;            // pieces of the pair, this one's number and workspace slot, slots between pieces
   FR_DEVI int block(int k) const { return k < nsb ? k : wb + k - nsb; }
 };
 // the tokens of one tile, as positions [pa, pb]
 struct Tile {
   int pa, pb, last, window, sinks;       // last: index of the last block that the tile needs (-1: none)
-  FR_DEVI Tile(const Item& it, int i, int tpt, int window_, int sinks_) : window(window_), sinks(sinks_) {
+  FR_DEVI Tile(const Item& it, int i, int tpt, int window_, int sinks_) : last(-1), window(window_), sinks(sinks_) {
     pa = it.pos0 + i * tpt;
     pb = min(it.pos0 + it.tok1 - it.tok0, pa + tpt) - 1;
-    last = pb >= max(pa, 0) ? it.nsb + pb / BN - it.wb : -1;
+    if (pb >= max(pa, 0))
+      for (int k = it.k1 - 1; k >= it.k0 && last < 0; --k)
+        if (needs(it.block(k) * BN)) last = k;
+    if (last < 0) pb = -1;                                     // nothing in this item's blocks
   }
-  FR_DEVI bool needs(int kb) const {
-    return last >= 0 && kb <= pb && (window <= 0 || kb + BN > pa - window + 1 || kb < sinks);
-  }
+  FR_DEVI bool needs(int kb) const { return kb <= pb && (window <= 0 || kb + BN > pa - window + 1 || kb < sinks); }
   FR_DEVI bool whole(int kb) const { return kb + BN - 1 <= pa && (window <= 0 || kb > pb - window || kb + BN <= sinks); }
 };
 
@@ -112,6 +118,24 @@ FR_DEVI float max3(float a, float b, float c) {
 // the n lowest of 32 bits
 FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
+FR_DEVI float4 f4(const uint32_t* v) {
+  return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+}
+template <int DT> FR_DEVI void put8(uint16_t* out, float4 x, float4 y, float inv, bool any) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (any) {
+    v.x = Elem<DT>::pack(x.x * inv, x.y * inv);
+    v.y = Elem<DT>::pack(x.z * inv, x.w * inv);
+    v.z = Elem<DT>::pack(y.x * inv, y.y * inv);
+    v.w = Elem<DT>::pack(y.z * inv, y.w * inv);
+  }
+  *reinterpret_cast<uint4*>(out) = v;
+}
+FR_DEVI void tile_sync(int i) {                                // the softmax warps of a tile
+  if (i == 0) asm volatile("bar.sync 1, 128;\n" ::: "memory");
+  else asm volatile("bar.sync 2, 128;\n" ::: "memory");
+}
+
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
                                                         const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
@@ -125,6 +149,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
                  pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base + S::MISC);
   volatile uint32_t* abort = tmem_slot + 1;
+  volatile uint32_t* flag = tmem_slot + 2;                     // [2]: this CTA joins the pieces of the tile
   Item* items = reinterpret_cast<Item*>(base + S::ITEMS);
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
 
@@ -166,8 +191,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     const int rows_all = static_cast<int>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh);
     const int nbox = BN / box_rows, box_sh = __ffs(box_rows) - 1;
     int n = 0, qc = 0;                                         // ring tiles and query pairs issued
-    // 32 sequences at a time: lane i has sequence r0 + i, its tokens, its items and the items up to and with it
-    int r0 = -32, beg = 0, end = 0;
+    // blocks of the pair at tok0 of a sequence with tokens up to end
+    const auto blocks = [&](int tok0, int end, int len, int& wb, int& nsb) {
+      const int pos0 = len - end + tok0, p1 = pos0 + min(2 * tpt, end - tok0) - 1;
+      const Span sp(max(pos0, 0), a.window, a.sinks);
+      wb = sp.lo / BN;
+      nsb = min((min(a.sinks, sp.lo) + BN - 1) / BN, wb);
+      return p1 >= 0 ? nsb + p1 / BN - wb + 1 : 0;
+    };
+    // blocks of the longest pair of a sequence: without a window the last pair's; with one the largest count that any pair
+    // can have (its keys span at most window + 2 tpt - 1 positions, which touch one block more than they fill)
+    const auto most_blocks = [&](int beg, int end, int len, int np) {
+      int wb, nsb;
+      const int last = blocks(beg + (np - 1) * 2 * tpt, end, len, wb, nsb);
+      return a.window <= 0 ? last : nsb + min((max(len, 1) - 1) / BN + 1, (min(a.window, 1 << 30) + 2 * tpt - 2) / BN + 2);
+    };
+    // few pairs: their key blocks are cut into pieces of `chunk` so that the grid is full, by the number of pieces that
+    // costs the least of max(one piece, waves of pieces); each piece of a pair has a workspace slot
+    int chunk = 1 << 30;
+    {
+      long long pairs = 0;
+      int most = 0;
+      float all = 0.f;
+      for (int b = lane; b < a.B; b += 32) {
+        const int beg = min(max(a.cu_q[b], 0), a.T), end = min(max(a.cu_q[b + 1], beg), a.T), len = a.c.len(b);
+        if (end == beg) continue;
+        const int np = (end - beg + 2 * tpt - 1) / (2 * tpt);
+        int x, y;
+        pairs += static_cast<long long>(np) * Hv;
+        most = max(most, most_blocks(beg, end, len, np));
+        all += 0.5f * (blocks(beg, end, len, x, y) + blocks(beg + (np - 1) * 2 * tpt, end, len, x, y)) * np * Hv;
+      }
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        pairs += __shfl_xor_sync(~0u, pairs, d);
+        most = max(most, __shfl_xor_sync(~0u, most, d));
+        all += __shfl_xor_sync(~0u, all, d);
+      }
+      if (pairs > 0 && 2 * pairs <= SLOTS && most > 1) {
+        const int sp = lane + 1, c = (most + sp - 1) / sp;     // lane i: i + 1 pieces
+        const float avg = all / static_cast<float>(pairs), per = ceilf(avg / c);
+        float cost = fmaxf(static_cast<float>(c + (sp > 1 ? SPLIT_COST : 0)),
+                           ceilf(pairs * per / gridDim.x) * (avg / fmaxf(per, 1.f) + (sp > 1 ? SPLIT_COST : 0)));
+        if (pairs * ((most + c - 1) / c) > SLOTS) cost = INFINITY;
+        float best = cost;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) best = fminf(best, __shfl_xor_sync(~0u, best, d));
+        const int at = __ffs(__ballot_sync(~0u, cost == best)) - 1;
+        if (at > 0) chunk = __shfl_sync(~0u, c, at);
+      }
+    }
+    // 32 sequences at a time: lane i has sequence r0 + i, its tokens, its items (pairs x pieces of the longest pair x heads)
+    // and the items up to and with it
+    int r0 = -32, beg = 0, end = 0, pieces = 1;
     long long mine = 0, upto = 0, row0 = 0, group = 0;         // row0: items before the 32
     long long idx = blockIdx.x;
     for (int ic = 0;; ++ic, idx += gridDim.x) {
@@ -182,7 +258,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           beg = min(max(a.cu_q[b], 0), a.T);
           end = min(max(a.cu_q[b + 1], beg), a.T);
         }
-        mine = static_cast<long long>((end - beg + 2 * tpt - 1) / (2 * tpt)) * Hv;
+        const int np = (end - beg + 2 * tpt - 1) / (2 * tpt);
+        pieces = 1;
+        if (chunk < 1 << 30 && np > 0) {
+          pieces = max((most_blocks(beg, end, a.c.len(b), np) + chunk - 1) / chunk, 1);
+        }
+        mine = static_cast<long long>(np) * pieces * Hv;
         upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -194,9 +275,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (r0 < a.B) {                                          // a head's pairs side by side, the longest first
         const int src = __ffs(__ballot_sync(~0u, row0 + upto > idx)) - 1, b = r0 + src;
         const int off = static_cast<int>(idx - row0 - __shfl_sync(~0u, upto - mine, src));
-        const int npairs = static_cast<int>(__shfl_sync(~0u, mine, src) / Hv);
-        const int sbeg = __shfl_sync(~0u, beg, src), send = __shfl_sync(~0u, end, src);
-        const int hv = off / npairs, pr = npairs - 1 - (off - hv * npairs);
+        const int sbeg = __shfl_sync(~0u, beg, src), send = __shfl_sync(~0u, end, src), np = __shfl_sync(~0u, pieces, src);
+        const int npairs = (send - sbeg + 2 * tpt - 1) / (2 * tpt);
+        const int hv = off / (npairs * np), rem = off - hv * npairs * np, part = rem / npairs, pr = npairs - 1 - (rem - part * npairs);
         it.b = b;
         it.h = hv / nhg;
         const int hg = hv - it.h * nhg;
@@ -206,11 +287,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         it.tok1 = min(it.tok0 + 2 * tpt, send);
         it.len = a.c.len(b);
         it.pos0 = it.len - send + it.tok0;
-        const int p1 = it.pos0 + it.tok1 - it.tok0 - 1;
-        const Span sp(max(it.pos0, 0), a.window, a.sinks);
-        it.wb = sp.lo / BN;
-        it.nsb = min((min(a.sinks, sp.lo) + BN - 1) / BN, it.wb);
-        it.nblk = p1 >= 0 ? it.nsb + p1 / BN - it.wb + 1 : 0;
+        const int nblk = blocks(it.tok0, send, it.len, it.wb, it.nsb);
+        it.k0 = part > 0 ? part * chunk : 0;
+        it.k1 = min(it.k0 + min(chunk, nblk), nblk);
+        it.ns = np > 1 ? max((nblk + chunk - 1) / chunk, 1) : 1;
+        it.part = part;
+        it.slot = static_cast<int>(idx);
+        it.stride = npairs;
+        if (part > 0 && it.k0 >= nblk) {                       // a shorter pair than the sequence's longest
+          --ic;
+          continue;
+        }
       }
       const int sl = ic & 1;
       if (ic >= 2 && !k16_wait(iempty + 8 * sl, (ic / 2 - 1) & 1)) break;
@@ -220,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       }
       __syncwarp();
       if (it.b < 0) break;
-      if (it.nblk == 0) continue;
+      if (it.k0 == it.k1) continue;
       // queries: [D half][token][head] = rows of 128 bytes; what lies outside q arrives as zeros
       if (qc > 0 && !k16_wait(qempty, (qc - 1) & 1)) break;
       if (lane == 0) {
@@ -232,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       ++qc;
       const int* bt = a.c.bt + it.b * a.c.bt_stride;
       bool ok = true;
-      for (int k = 0; k < it.nblk && ok; ++k) {
+      for (int k = it.k0; k < it.k1 && ok; ++k) {
         const int j = it.block(k) * BN + lane * box_rows;      // lane i < nbox: box i of the block
         int y = rows_all;
         if (lane < nbox && j < it.len) {
@@ -276,17 +363,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       __syncwarp();
       if (lane == 0) tc5::mbar_arrive(iempty + 8 * sl);
       if (it.b < 0) break;
-      if (it.nblk == 0) continue;
+      if (it.k0 == it.k1) continue;
       const Tile t0(it, 0, tpt, a.window, a.sinks), t1(it, 1, tpt, a.window, a.sinks);
       if (!k16_wait(qfull, qc & 1)) break;
       ++qc;
       tc5::fence_after_sync();
       bool started[2] = {false, false};
-      for (int k = 0; k <= it.nblk && run; ++k) {
-        const int nv = n + 2 * k - 1, nk = n + 2 * k;          // ring tiles of V(k - 1) and K(k)
+      for (int k = it.k0; k <= it.k1 && run; ++k) {
+        const int nv = n + 2 * (k - it.k0) - 1, nk = nv + 1;          // ring tiles of V(k - 1) and K(k)
         const uint32_t sv = sm + S::RING + (nv % STAGES) * S::STAGE, sk = sm + S::RING + (nk % STAGES) * S::STAGE;
-        const int kbv = k > 0 ? it.block(k - 1) * BN : 0, kbk = k < it.nblk ? it.block(k) * BN : 0;
-        if (k > 0) {
+        const int kbv = k > it.k0 ? it.block(k - 1) * BN : 0, kbk = k < it.k1 ? it.block(k) * BN : 0;
+        if (k > it.k0) {
           if (!(run = k16_wait(full + 8 * (nv % STAGES), (nv / STAGES) & 1))) break;
           if (kbv + BN > it.len) {                             // values behind the sequence: 0 * NaN would be NaN
             for (int i = (it.len - kbv) * 8 + lane; i < BN * 8; i += 32)
@@ -301,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const Tile& t = i ? t1 : t0;
-          if (k > 0 && t.needs(kbv)) {
+          if (k > it.k0 && t.needs(kbv)) {
             if (!(run = k16_wait(pfull + 8 * i, pc[i] & 1))) break;
             ++pc[i];
             tc5::fence_after_sync();
@@ -314,12 +401,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
             __syncwarp();
             started[i] = true;
           }
-          if (k < it.nblk && !have_k) {
+          if (k < it.k1 && !have_k) {
             if (!(run = k16_wait(full + 8 * (nk % STAGES), (nk / STAGES) & 1))) break;
             have_k = true;
             tc5::fence_after_sync();
           }
-          if (k < it.nblk && t.needs(kbk)) {
+          if (k < it.k1 && t.needs(kbk)) {
             if (tc5::elect_one()) {
 #pragma unroll
               for (int s = 0; s < D / 16; ++s)
@@ -332,13 +419,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         }
         if (!run) break;
         if (tc5::elect_one()) {
-          if (k > 0) tc5::mma_commit(empty + 8 * (nv % STAGES));
-          if (k < it.nblk) tc5::mma_commit(empty + 8 * (nk % STAGES));
-          if (k == it.nblk - 1) tc5::mma_commit(qempty);
+          if (k > it.k0) tc5::mma_commit(empty + 8 * (nv % STAGES));
+          if (k < it.k1) tc5::mma_commit(empty + 8 * (nk % STAGES));
+          if (k == it.k1 - 1) tc5::mma_commit(qempty);
         }
         __syncwarp();
       }
-      n += 2 * it.nblk;
+      n += 2 * (it.k1 - it.k0);
     }
   } else {                                                     // --------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFT));
@@ -362,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       const bool live = tok < tpt && head < it.heads && mytok < it.tok1;
       const int pos = live ? it.pos0 + i * tpt + tok : -1;
       float ref = -INFINITY, l = 0.f;
-      for (int k = 0; k < it.nblk; ++k) {
+      for (int k = it.k0; k < it.k1; ++k) {
         const int kb = it.block(k) * BN;
         if (!t.needs(kb)) continue;
         if (!(run = k16_wait(sfull + 8 * i, sc & 1))) break;
@@ -399,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           // S(k) is complete, so every product into O before it is; the next one waits for this P
           if (__any_sync(~0u, l > 0.f)) {
             l *= f;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tc5::tmem_ld32(to + 32 * c, o);
@@ -442,29 +529,85 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         ++oc;
         tc5::fence_after_sync();
       }
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;     // a row that sees nothing gives zeros; NaN stays NaN
       uint16_t* out = static_cast<uint16_t*>(a.out) + mytok * a.o_ts + (it.hq0 + head) * D;
+      if (it.ns == 1) {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // a row that sees nothing gives zeros; NaN stays NaN
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (any) {
-          tc5::tmem_ld32(to + 32 * c, o);
-          tc5::tmem_ld_wait();
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (any) {
+            tc5::tmem_ld32(to + 32 * c, o);
+            tc5::tmem_ld_wait();
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) put8<DT>(out + 32 * c + e, f4(o + e), f4(o + e + 4), inv, any && inv != 0.f);
+          }
+          __syncwarp();
         }
-        if (live) {
+      } else {
+        // this piece's sums to its slot, [dims / 4][row] x 16 bytes; the last piece of the tile to arrive joins them in order
+        const int rr = i * (D / 4) * 128 + r;
+        float4* po = reinterpret_cast<float4*>(a.ws) + static_cast<long long>(it.slot) * (2 * (D / 4) * 128) + rr;
+        float2* pl = reinterpret_cast<float2*>(a.ws + static_cast<long long>(SLOTS) * (2 * D * 128 * 4));
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (any && inv != 0.f) {
-              x.x = Elem<DT>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              x.y = Elem<DT>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              x.z = Elem<DT>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              x.w = Elem<DT>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            }
-            *reinterpret_cast<uint4*>(out + 32 * c + e) = x;
+        for (int c = 0; c < D / 32; ++c) {
+          if (any) {
+            uint32_t o[32];
+            tc5::tmem_ld32(to + 32 * c, o);
+            tc5::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) __stcg(po + (c * 8 + e) * 128, f4(o + 4 * e));
           }
         }
-        __syncwarp();
+        __stcg(pl + static_cast<long long>(it.slot) * 256 + i * 128 + r, make_float2(ref, l));
+        __threadfence();
+        tile_sync(i);
+        const int slot0 = it.slot - it.part * it.stride;
+        if (r == 0) {
+          int* tk = a.tickets + 2 * slot0 + i;
+          const int old = atomicAdd(tk, 1);
+          if (old == it.ns - 1) *tk = 0;
+          flag[i] = old == it.ns - 1;
+          __threadfence();
+        }
+        tile_sync(i);
+        if (flag[i]) {
+          const float2* ml = pl + static_cast<long long>(slot0) * 256 + i * 128 + r;
+          const float4* pq = reinterpret_cast<const float4*>(a.ws) + static_cast<long long>(slot0) * (2 * (D / 4) * 128) + rr;
+          float M = -INFINITY, L = 0.f;
+          for (int s = 0; s < it.ns; ++s) M = fmaxf(M, __ldcg(ml + static_cast<long long>(s * it.stride) * 256).x);
+          for (int s = 0; s < it.ns; ++s) {
+            const float2 e = __ldcg(ml + static_cast<long long>(s * it.stride) * 256);
+            if (e.y != 0.f) L = fmaf(ex2(e.x - M), e.y, L);    // (0: the piece has no key that this row sees)
+          }
+          const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+#pragma unroll 1
+          for (int c = 0; c < D / 4; c += 8) {
+            float4 acc[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < it.ns; ++s) {
+              const float2 e2 = __ldcg(ml + static_cast<long long>(s * it.stride) * 256);
+              if (e2.y == 0.f) continue;
+              const float f = ex2(e2.x - M);
+              const float4* q = pq + static_cast<long long>(s * it.stride) * (2 * (D / 4) * 128) + c * 128;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float4 x = __ldcg(q + e * 128);
+                acc[e].x = fmaf(f, x.x, acc[e].x);
+                acc[e].y = fmaf(f, x.y, acc[e].y);
+                acc[e].z = fmaf(f, x.z, acc[e].z);
+                acc[e].w = fmaf(f, x.w, acc[e].w);
+              }
+            }
+            if (live)
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) put8<DT>(out + 4 * (c + e), acc[e], acc[e + 1], inv, inv != 0.f);
+          }
+          __syncwarp();
+        }
+        tile_sync(i);                                          // (the flag is free again)
       }
       tc5::fence_before_sync();
     }
@@ -487,8 +630,20 @@ cudaError_t launch(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMa
 
 }  // namespace
 
-long long prefill_ws_bytes(int, int, int, int, long long) { return 0; }
-long long prefill_tickets(int, int, int, long long) { return 0; }
+static void groups(int G, int& nhg, int& hb, int& tpt) {       // q heads per item, tokens per tile
+  nhg = (G + MAX_HEADS - 1) / MAX_HEADS;
+  hb = (G + nhg - 1) / nhg;
+  tpt = 128 / hb;
+}
+// pairs at most: every sequence may end inside one
+static long long max_pairs(int rows, int Hkv, int G, long long new_tokens) {
+  int nhg, hb, tpt;
+  groups(G, nhg, hb, tpt);
+  return (new_tokens / (2 * tpt) + rows) * Hkv * nhg;
+}
+// sums and (reference, denominator) of every slot; a pair is split into MAX_SPLIT pieces at most
+long long prefill_ws_bytes(int, int, int, int D, long long) { return static_cast<long long>(SLOTS) * 256 * (D * 4 + 8); }
+long long prefill_tickets(int, int, int, long long) { return 2 * SLOTS; }
 
 int prefill_status() {
   int v = -1;
@@ -500,15 +655,16 @@ cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  const int nhg = (a.G + MAX_HEADS - 1) / MAX_HEADS, hb = (a.G + nhg - 1) / nhg, tpt = 128 / hb, Hq = a.c.Hkv * a.G;
+  int nhg, hb, tpt;
+  groups(a.G, nhg, hb, tpt);
+  const int Hq = a.c.Hkv * a.G;
   const int box = 1 << a.c.page_sh;                            // page <= 128 = BN rows
   CUtensorMap qm, kv;
   e = encode4(&qm, dtype, a.q, Hq, a.D * 2ull, a.T, a.T > 1 ? a.q_ts * 2ull : Hq * a.D * 2ull, a.D / 64, 128, hb, tpt);
   if (e == cudaSuccess)
     e = encode3(&kv, dtype, a.c.pool, static_cast<uint64_t>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh), a.D * 2ull, a.D / 64, 128, box, 1);
   if (e != cudaSuccess) return e;
-  // items at most: every sequence may end inside a pair
-  const long long items = (static_cast<long long>(a.T) / (2 * tpt) + a.B) * a.c.Hkv * nhg;
+  const long long items = max_pairs(a.B, a.c.Hkv, a.G, a.T) * MAX_SPLIT;
   const int grid = static_cast<int>(items < sms ? items : sms);
   if (dtype == 0)
     return a.D == 128 ? launch<0, 128>(a, qm, kv, hb, nhg, box, grid, st) : launch<0, 64>(a, qm, kv, hb, nhg, box, grid, st);
