@@ -7,9 +7,10 @@
 // kv head): rows are tokens times the G q heads of the group, so all heads of a group share every key and value tile that is
 // fetched.  S (128 keys at a time), P and O of both tiles live in tensor memory (512 columns: S0 S1 O0 O1, P over its own S).
 //
-// CTA (one per SM, persistent): warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread per row), warp 8 issues the
-// MMAs, warp 9 takes work items and issues the tensor copies (Q once per item, K and V tiles of 128 keys through one ring).
-// The tensor pipe alternates  P0 V(j-1), Q0 K(j), P1 V(j-1), Q1 K(j):  while one tile's softmax runs, the other's products do.
+// CTA (one per SM, persistent): warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread per row), warps 8 and 9
+// issue the MMAs of tile 0 and 1 (P V(j-1), then Q K(j)), warp 10 takes work items and issues the tensor copies (Q once per
+// item, K and V tiles of 128 keys through one ring).  The tiles run half a step apart: while one's softmax runs, the tensor
+// pipe has the other's products.  A warp per tile because a step costs an issuing warp some hundred cycles between its MMAs.
 // The softmax reference is lazy: it moves when a row's maximum has grown by more than 2^8, and only then is O rescaled.
 //
 // V is taken as it lies (keys by dims): the second product's B operand is MN-major, K = keys.
@@ -22,13 +23,14 @@ namespace k16 {
 namespace {
 
 constexpr int BN = 128;                  // keys per block
-constexpr int THREADS = 384;            // three warpgroups: two of softmax, one of MMA, copies and two idle warps
-constexpr int W_MMA = 8, W_TMA = 9;
+constexpr int THREADS = 384;            // three warpgroups: two of softmax, one of MMA (a warp per tile), copies and an idle warp
+constexpr int W_MMA = 8, W_TMA = 10;
 constexpr int REGS_SOFT = 216, REGS_REST = 72;   // 256 x 216 + 128 x 72 = 384 x 168, what the launch has
 constexpr int MAX_HEADS = 128;           // q heads per item
 constexpr float LAZY = 8.f;
+constexpr float SEEN = 1e-20f;           // a row that has seen a key has a sum of about 1 at least
 constexpr int MAX_SPLIT = 32;            // pieces of a pair's key blocks
-constexpr int SLOTS = 2 * 148;           // workspace slots: pieces of split pairs
+constexpr int SLOTS = 4 * 148;           // workspace slots: pieces of split pairs
 constexpr int SPLIT_COST = 4;            // what a piece costs besides its blocks, in blocks
 
 __device__ int g_status;
@@ -63,8 +65,8 @@ template <int D> struct Smem {
   static constexpr int STAGE = BN * D * 2;                     // one K or V tile
   static constexpr int STAGES = D == 128 ? 5 : 10;
   static constexpr int RING = 2 * QT;
-  static constexpr int BAR = RING + STAGES * STAGE;            // full[STAGES] empty[STAGES] qfull qempty sfull[2] pfull[2] ofull[2]
-  static constexpr int NBAR = 2 * STAGES + 2 + 6 + 4;          // ... items: full[2], empty[2]
+  static constexpr int BAR = RING + STAGES * STAGE;            // full[STAGES] empty[STAGES] qfull qempty sfull[2] pfull[2][2] ofull[2]
+  static constexpr int NBAR = 2 * STAGES + 2 + 8 + 4 + 2;          // ... items: full[2], empty[2]; tile sync[2]
   static constexpr int ITEMS = BAR + NBAR * 8;                 // Item[2]
   static constexpr int MISC = ITEMS + 2 * 64;                  // tensor-memory base, abort flag
   static constexpr int TOTAL = MISC + 16 + 1024;
@@ -82,12 +84,26 @@ FR_DEVI bool wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort, in
 }
 #define k16_wait(bar, parity) wait_at(bar, parity, abort, __LINE__)
 
-// MN-major operand in 128-byte swizzle: lbo = bytes between 64-element chunks along N, sbo = bytes between groups of 8 keys
-FR_DEVI uint64_t desc_mn(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return tc5::DESC_VERSION | tc5::DESC_SW128 | (static_cast<uint64_t>(sbo >> 4) << 32) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-         ((saddr & 0x3FFFFu) >> 4);
+// Operand descriptors in 128-byte swizzle as two words, of which only the low one (the address) changes: K-major with 1024
+// bytes between groups of 8 rows; MN-major (V) with BN * 128 bytes between 64-dim chunks and 1024 between groups of 8 keys.
+constexpr uint32_t DESC_HI = static_cast<uint32_t>((tc5::DESC_VERSION | tc5::DESC_SW128) >> 32) | (1024 >> 4);
+constexpr uint32_t DESC_LO_K = 1u << 16, DESC_LO_MN = static_cast<uint32_t>(BN * 128 >> 4) << 16;
+FR_DEVI uint32_t desc_lo(uint32_t saddr, uint32_t bits) { return bits | ((saddr & 0x3FFFFu) >> 4); }
+FR_DEVI void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(accumulate), "n"(DESC_HI)
+      : "memory");
 }
-constexpr uint32_t B_MN_MAJOR = 1u << 16;                      // instruction descriptor: B is MN-major
+FR_DEVI void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(accumulate), "n"(DESC_HI)
+      : "memory");
+}
+constexpr uint32_t A_NEGATE = 1u << 13, B_MN_MAJOR = 1u << 16;  // bits of the instruction descriptor
 
 // two floats in one register pair; each half is rounded like the scalar operation
 FR_DEVI uint64_t pk(float x, float y) {
@@ -131,11 +147,6 @@ template <int DT> FR_DEVI void put8(uint16_t* out, float4 x, float4 y, float inv
   }
   *reinterpret_cast<uint4*>(out) = v;
 }
-FR_DEVI void tile_sync(int i) {                                // the softmax warps of a tile
-  if (i == 0) asm volatile("bar.sync 1, 128;\n" ::: "memory");
-  else asm volatile("bar.sync 2, 128;\n" ::: "memory");
-}
-
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
                                                         const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
@@ -146,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
   const uint32_t sm = (raw + 1023) & ~1023u;
   unsigned char* base = smem_raw + (sm - raw);
   const uint32_t full = sm + S::BAR, empty = full + 8 * STAGES, qfull = empty + 8 * STAGES, qempty = qfull + 8, sfull = qempty + 8,
-                 pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16;
+                 pfull = sfull + 16, ofull = pfull + 32, ifull = ofull + 16, iempty = ifull + 16, tsync = iempty + 16;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base + S::MISC);
   volatile uint32_t* abort = tmem_slot + 1;
   volatile uint32_t* flag = tmem_slot + 2;                     // [2]: this CTA joins the pieces of the tile
@@ -156,16 +167,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       tc5::mbar_init(full + 8 * i, 1);
-      tc5::mbar_init(empty + 8 * i, 1);
+      tc5::mbar_init(empty + 8 * i, 2);
     }
     tc5::mbar_init(qfull, 1);
-    tc5::mbar_init(qempty, 1);
+    tc5::mbar_init(qempty, 2);
     for (int i = 0; i < 2; ++i) {
       tc5::mbar_init(sfull + 8 * i, 1);
-      tc5::mbar_init(pfull + 8 * i, 4);
+      tc5::mbar_init(pfull + 16 * i, 4);
+      tc5::mbar_init(pfull + 16 * i + 8, 4);
       tc5::mbar_init(ofull + 8 * i, 1);
       tc5::mbar_init(ifull + 8 * i, 1);
-      tc5::mbar_init(iempty + 8 * i, 9);
+      tc5::mbar_init(tsync + 8 * i, 4);
+      tc5::mbar_init(iempty + 8 * i, 10);
     }
     tc5::mbar_init_fence();
     *abort = 0;
@@ -199,56 +212,52 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       nsb = min((min(a.sinks, sp.lo) + BN - 1) / BN, wb);
       return p1 >= 0 ? nsb + p1 / BN - wb + 1 : 0;
     };
-    // blocks of the longest pair of a sequence: without a window the last pair's; with one the largest count that any pair
-    // can have (its keys span at most window + 2 tpt - 1 positions, which touch one block more than they fill)
-    const auto most_blocks = [&](int beg, int end, int len, int np) {
-      int wb, nsb;
-      const int last = blocks(beg + (np - 1) * 2 * tpt, end, len, wb, nsb);
-      return a.window <= 0 ? last : nsb + min((max(len, 1) - 1) / BN + 1, (min(a.window, 1 << 30) + 2 * tpt - 2) / BN + 2);
-    };
-    // few pairs: their key blocks are cut into pieces of `chunk` so that the grid is full, by the number of pieces that
-    // costs the least of max(one piece, waves of pieces); each piece of a pair has a workspace slot
-    int chunk = 1 << 30;
-    {
-      long long pairs = 0;
-      int most = 0;
-      float all = 0.f;
-      for (int b = lane; b < a.B; b += 32) {
-        const int beg = min(max(a.cu_q[b], 0), a.T), end = min(max(a.cu_q[b + 1], beg), a.T), len = a.c.len(b);
-        if (end == beg) continue;
-        const int np = (end - beg + 2 * tpt - 1) / (2 * tpt);
-        int x, y;
-        pairs += static_cast<long long>(np) * Hv;
-        most = max(most, most_blocks(beg, end, len, np));
-        all += 0.5f * (blocks(beg, end, len, x, y) + blocks(beg + (np - 1) * 2 * tpt, end, len, x, y)) * np * Hv;
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        pairs += __shfl_xor_sync(~0u, pairs, d);
-        most = max(most, __shfl_xor_sync(~0u, most, d));
-        all += __shfl_xor_sync(~0u, all, d);
-      }
-      if (pairs > 0 && 2 * pairs <= SLOTS && most > 1) {
-        const int sp = lane + 1, c = (most + sp - 1) / sp;     // lane i: i + 1 pieces
-        const float avg = all / static_cast<float>(pairs), per = ceilf(avg / c);
-        float cost = fmaxf(static_cast<float>(c + (sp > 1 ? SPLIT_COST : 0)),
-                           ceilf(pairs * per / gridDim.x) * (avg / fmaxf(per, 1.f) + (sp > 1 ? SPLIT_COST : 0)));
-        if (pairs * ((most + c - 1) / c) > SLOTS) cost = INFINITY;
-        float best = cost;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) best = fminf(best, __shfl_xor_sync(~0u, best, d));
-        const int at = __ffs(__ballot_sync(~0u, cost == best)) - 1;
-        if (at > 0) chunk = __shfl_sync(~0u, c, at);
-      }
+    // The list: all pairs; those of the last, partly filled wave are cut into `split` pieces by their key blocks (the number
+    // that costs least: waves of pieces times a piece), each with a workspace slot, so that the whole grid ends together.
+    long long pairs = 0;
+    float all = 0.f;
+    for (int b = lane; b < a.B; b += 32) {
+      const int beg = min(max(a.cu_q[b], 0), a.T), end = min(max(a.cu_q[b + 1], beg), a.T), len = a.c.len(b);
+      if (end == beg) continue;
+      const int np = (end - beg + 2 * tpt - 1) / (2 * tpt);
+      int x, y;
+      pairs += static_cast<long long>(np) * Hv;
+      all += 0.5f * (blocks(beg, end, len, x, y) + blocks(beg + (np - 1) * 2 * tpt, end, len, x, y)) * np * Hv;
     }
-    // 32 sequences at a time: lane i has sequence r0 + i, its tokens, its items (pairs x pieces of the longest pair x heads)
-    // and the items up to and with it
-    int r0 = -32, beg = 0, end = 0, pieces = 1;
-    long long mine = 0, upto = 0, row0 = 0, group = 0;         // row0: items before the 32
-    long long idx = blockIdx.x;
-    for (int ic = 0;; ++ic, idx += gridDim.x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      pairs += __shfl_xor_sync(~0u, pairs, d);
+      all += __shfl_xor_sync(~0u, all, d);
+    }
+    const int rest = static_cast<int>(pairs % gridDim.x);
+    const long long whole = pairs - rest;
+    int split = 1;
+    if (rest > 0) {
+      const int sp = lane + 1;                                 // lane i: i + 1 pieces
+      const float avg = all / static_cast<float>(pairs), n = ceilf(fminf(avg, static_cast<float>(sp)));
+      float cost = ceilf(rest * n / gridDim.x) * (avg / n + (sp > 1 ? SPLIT_COST : 0));
+      if (rest * sp > SLOTS || avg < 1.f) cost = sp == 1 ? 1e30f : INFINITY;
+      float best = cost;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) best = fminf(best, __shfl_xor_sync(~0u, best, d));
+      split = __ffs(__ballot_sync(~0u, cost == best));
+    }
+    const long long units = whole + static_cast<long long>(rest) * split;
+    // 32 sequences at a time: lane i has sequence r0 + i, its tokens, its pairs (times heads) and the pairs up to and with it
+    int r0 = -32, beg = 0, end = 0;
+    long long mine = 0, upto = 0, row0 = 0, group = 0;         // row0: pairs before the 32
+    long long unit = blockIdx.x, before = -1;
+    for (int ic = 0;; ++ic, unit += gridDim.x) {
       Item it;
       it.b = -1;
+      const int extra = static_cast<int>(max(unit - whole, 0ll));
+      const int part = rest > 0 ? extra / rest : 0;
+      const long long idx = unit < whole ? unit : unit < units ? whole + extra - part * rest : pairs;
+      if (idx < before) {                                      // the next pieces of the last pairs: from the front again
+        r0 = -32;
+        row0 = group = 0;
+      }
+      before = idx;
       while (r0 < a.B && idx >= row0 + group) {                // (indices only grow)
         row0 += group;
         r0 += 32;
@@ -258,12 +267,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           beg = min(max(a.cu_q[b], 0), a.T);
           end = min(max(a.cu_q[b + 1], beg), a.T);
         }
-        const int np = (end - beg + 2 * tpt - 1) / (2 * tpt);
-        pieces = 1;
-        if (chunk < 1 << 30 && np > 0) {
-          pieces = max((most_blocks(beg, end, a.c.len(b), np) + chunk - 1) / chunk, 1);
-        }
-        mine = static_cast<long long>(np) * pieces * Hv;
+        mine = static_cast<long long>((end - beg + 2 * tpt - 1) / (2 * tpt)) * Hv;
         upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -275,9 +279,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (r0 < a.B) {                                          // a head's pairs side by side, the longest first
         const int src = __ffs(__ballot_sync(~0u, row0 + upto > idx)) - 1, b = r0 + src;
         const int off = static_cast<int>(idx - row0 - __shfl_sync(~0u, upto - mine, src));
-        const int sbeg = __shfl_sync(~0u, beg, src), send = __shfl_sync(~0u, end, src), np = __shfl_sync(~0u, pieces, src);
+        const int sbeg = __shfl_sync(~0u, beg, src), send = __shfl_sync(~0u, end, src);
         const int npairs = (send - sbeg + 2 * tpt - 1) / (2 * tpt);
-        const int hv = off / (npairs * np), rem = off - hv * npairs * np, part = rem / npairs, pr = npairs - 1 - (rem - part * npairs);
+        const int hv = off / npairs, pr = npairs - 1 - (off - hv * npairs);
         it.b = b;
         it.h = hv / nhg;
         const int hg = hv - it.h * nhg;
@@ -288,13 +292,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         it.len = a.c.len(b);
         it.pos0 = it.len - send + it.tok0;
         const int nblk = blocks(it.tok0, send, it.len, it.wb, it.nsb);
-        it.k0 = part > 0 ? part * chunk : 0;
-        it.k1 = min(it.k0 + min(chunk, nblk), nblk);
-        it.ns = np > 1 ? max((nblk + chunk - 1) / chunk, 1) : 1;
+        const int sp = unit < whole ? 1 : max(min(split, nblk), 1), chunk = (nblk + sp - 1) / sp;
+        it.k0 = min(part * chunk, nblk);
+        it.k1 = min(it.k0 + chunk, nblk);
+        it.ns = nblk > 0 ? (nblk + chunk - 1) / chunk : 1;
         it.part = part;
-        it.slot = static_cast<int>(idx);
-        it.stride = npairs;
-        if (part > 0 && it.k0 >= nblk) {                       // a shorter pair than the sequence's longest
+        it.slot = extra;
+        it.stride = rest;
+        if (part > 0 && it.k0 >= nblk) {                       // a pair of fewer blocks than pieces
           --ic;
           continue;
         }
@@ -351,10 +356,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       tc5::mbar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1);
     }
     if (*abort && lane == 0 && qc) tc5::mbar_wait(qfull, (qc - 1) & 1);
-  } else if (w == W_MMA) {                                     // ------------------------------------------------------ MMAs
-    constexpr uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, BN);
+  } else if (w == W_MMA || w == W_MMA + 1) {                   // ------------------------------------- MMAs, a warp per tile
+    // the softmax takes |qscale|: a negative scale negates the A operand
+    const uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, BN) | (a.qscale < 0.f ? A_NEGATE : 0u);
     constexpr uint32_t ID_PV = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, D) | B_MN_MAJOR;
-    int n = 0, qc = 0, pc[2] = {0, 0};                         // ring tiles, query pairs, P tiles consumed
+    const int i = w - W_MMA;
+    const uint32_t tSi = tS + i * 128, tOi = tO + i * 128, qlo = desc_lo(sm + i * S::QT, DESC_LO_K), pf = pfull + 16 * i;
+    int qc = 0, pc = 0;                                        // query pairs and P tiles consumed
+    int st = 0, ph = 0;                                        // the ring's next tile: K(k0), V(k0), K(k0 + 1), ... of every item
     bool run = true;
     for (int ic = 0; run; ++ic) {
       const int sl = ic & 1;
@@ -364,77 +373,88 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (lane == 0) tc5::mbar_arrive(iempty + 8 * sl);
       if (it.b < 0) break;
       if (it.k0 == it.k1) continue;
-      const Tile t0(it, 0, tpt, a.window, a.sinks), t1(it, 1, tpt, a.window, a.sinks);
+      const Tile t(it, i, tpt, a.window, a.sinks);
       if (!k16_wait(qfull, qc & 1)) break;
       ++qc;
       tc5::fence_after_sync();
-      bool started[2] = {false, false};
-      for (int k = it.k0; k <= it.k1 && run; ++k) {
-        const int nv = n + 2 * (k - it.k0) - 1, nk = nv + 1;          // ring tiles of V(k - 1) and K(k)
-        const uint32_t sv = sm + S::RING + (nv % STAGES) * S::STAGE, sk = sm + S::RING + (nk % STAGES) * S::STAGE;
-        const int kbv = k > it.k0 ? it.block(k - 1) * BN : 0, kbk = k < it.k1 ? it.block(k) * BN : 0;
+      bool was = false, begun = false;                         // the tile needs V(k - 1); its O has begun
+      int kbv = 0;                                             // first key of block k - 1
+      for (int k = it.k0; k <= it.k1; ++k) {
+        const int kb = k < it.k1 ? it.block(k) * BN : 0;
+        const bool now = k < it.k1 && t.needs(kb);
+        // Every tile of the ring is waited for, needed or not: the parity of a later phase would not tell.
         if (k > it.k0) {
-          if (!(run = k16_wait(full + 8 * (nv % STAGES), (nv / STAGES) & 1))) break;
-          if (kbv + BN > it.len) {                             // values behind the sequence: 0 * NaN would be NaN
-            for (int i = (it.len - kbv) * 8 + lane; i < BN * 8; i += 32)
+          const uint32_t sv = sm + S::RING + st * S::STAGE, vlo = desc_lo(sv, DESC_LO_MN), vbar = empty + 8 * st;
+          if (!(run = k16_wait(full + 8 * st, ph))) break;
+          if (++st == STAGES) st = 0, ph ^= 1;
+          if (was) {
+            if (kbv + BN > it.len) {                           // values behind the sequence: 0 * NaN would be NaN
+              for (int j = (it.len - kbv) * 8 + lane; j < BN * 8; j += 32)
 #pragma unroll
-              for (int x = 0; x < HALVES; ++x)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + i * 16), "r"(0) : "memory");
-            tc5::fence_async_smem();
-            __syncwarp();
+                for (int x = 0; x < HALVES; ++x)
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + j * 16), "r"(0) : "memory");
+              tc5::fence_async_smem();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {                      // P comes in two halves of 64 keys
+              if (!(run = k16_wait(pf + 8 * c, pc & 1))) break;
+              tc5::fence_after_sync();
+              if (tc5::elect_one()) {
+#pragma unroll
+                for (int s = 4 * c; s < 4 * c + 4; ++s)
+                  mma_ts(tOi, tSi + s * 8, vlo + s * (2048 >> 4), ID_PV, s > 0 ? 1u : static_cast<uint32_t>(begun));
+                if (c == 1) tc5::mma_commit(vbar);
+                if (c == 1 && k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
+              }
+              __syncwarp();
+            }
+            if (!run) break;
+            ++pc;
+            begun = true;
+          } else if (lane == 0) {
+            tc5::mbar_arrive(vbar);
           }
         }
-        bool have_k = false;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const Tile& t = i ? t1 : t0;
-          if (k > it.k0 && t.needs(kbv)) {
-            if (!(run = k16_wait(pfull + 8 * i, pc[i] & 1))) break;
-            ++pc[i];
-            tc5::fence_after_sync();
-            if (tc5::elect_one()) {
-#pragma unroll
-              for (int s = 0; s < BN / 16; ++s)
-                tc5::mma_f16_ts(tO + i * 128, tS + i * 128 + s * 8, desc_mn(sv + s * 2048, BN * 128, 1024), ID_PV, started[i] || s > 0);
-              if (k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
-            }
-            __syncwarp();
-            started[i] = true;
-          }
-          if (k < it.k1 && !have_k) {
-            if (!(run = k16_wait(full + 8 * (nk % STAGES), (nk / STAGES) & 1))) break;
-            have_k = true;
-            tc5::fence_after_sync();
-          }
-          if (k < it.k1 && t.needs(kbk)) {
+        if (k < it.k1) {
+          const uint32_t klo = desc_lo(sm + S::RING + st * S::STAGE, DESC_LO_K), kbar = empty + 8 * st;
+          if (!(run = k16_wait(full + 8 * st, ph))) break;
+          if (++st == STAGES) st = 0, ph ^= 1;
+          tc5::fence_after_sync();
+          if (now) {
             if (tc5::elect_one()) {
 #pragma unroll
               for (int s = 0; s < D / 16; ++s)
-                tc5::mma_f16_ss(tS + i * 128, tc5::desc_sw128(sm + i * S::QT + (s >> 2) * 128 * 128 + (s & 3) * 32, 1024),
-                                tc5::desc_sw128(sk + (s >> 2) * BN * 128 + (s & 3) * 32, 1024), ID_QK, s > 0);
+                mma_ss(tSi, qlo + (((s >> 2) * 128 * 128 + (s & 3) * 32) >> 4), klo + (((s >> 2) * BN * 128 + (s & 3) * 32) >> 4), ID_QK, s > 0);
               tc5::mma_commit(sfull + 8 * i);
+              tc5::mma_commit(kbar);
+              if (k == it.k1 - 1) tc5::mma_commit(qempty);
             }
+            __syncwarp();
+          } else if (lane == 0) {
+            tc5::mbar_arrive(kbar);
+          }
+          if (!now && k == it.k1 - 1) {                        // (this tile's last product was an earlier block's)
+            if (tc5::elect_one()) tc5::mma_commit(qempty);
             __syncwarp();
           }
         }
-        if (!run) break;
-        if (tc5::elect_one()) {
-          if (k > it.k0) tc5::mma_commit(empty + 8 * (nv % STAGES));
-          if (k < it.k1) tc5::mma_commit(empty + 8 * (nk % STAGES));
-          if (k == it.k1 - 1) tc5::mma_commit(qempty);
-        }
-        __syncwarp();
+        was = now, kbv = kb;
       }
-      n += 2 * (it.k1 - it.k0);
     }
   } else {                                                     // --------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFT));
     const int i = w >> 2, r = tid & 127, tok = r / hb, head = r - tok * hb;
     const uint32_t lanes = static_cast<uint32_t>(w & 3) << 21;  // tensor-memory lanes of this warp
     const uint32_t ts = tS + i * 128 + lanes, to = tO + i * 128 + lanes;
-    const bool neg = a.qscale < 0.f;                           // the maximum is taken of |qscale| (+-S)
     const float qs = fmaxf(fabsf(a.qscale), 1e-37f);           // a scale of 0: all scores alike, and -inf * qs stays -inf
     constexpr float BIAS = DT == 1 ? 6.f : 0.f;                // fp16 weights are carried times 2^6: their steps below 2^-14 are absolute
+    int syncs = 0;
+    const auto tile_sync = [&]() {                             // the softmax warps of a tile (bounded, unlike a named barrier)
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(tsync + 8 * i);
+      return k16_wait(tsync + 8 * i, syncs++ & 1);
+    };
     int sc = 0, oc = 0;                                        // S and O tiles consumed
     bool run = true;
     for (int ic = 0; run; ++ic) {
@@ -459,10 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < 4; ++c) tc5::tmem_ld32(ts + 32 * c, v[c]);
         tc5::tmem_ld_wait();
-        if (neg)
-#pragma unroll
-          for (int c = 0; c < 128; ++c) v[c >> 5][c & 31] ^= 0x80000000u;
-        if (!t.whole(kb)) {
+        if (__builtin_expect(!t.whole(kb), 0)) {
           const int hi = pos + 1 - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : 0, sk = a.sinks - kb;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -481,11 +498,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           m3 = max3(m3, __uint_as_float(v[3][c]), __uint_as_float(v[3][c + 1]));
         }
         const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
-        if (__any_sync(~0u, m > ref + LAZY)) {
+        if (__builtin_expect(__any_sync(~0u, m > ref + LAZY), 0)) {
           const float nr = fmaxf(m, ref), f = ref == -INFINITY ? 0.f : ex2(ref - nr);
           // S(k) is complete, so every product into O before it is; the next one waits for this P
-          if (__any_sync(~0u, l > 0.f)) {
-            l *= f;
+          const bool some = l > SEEN;
+          l *= f;
+          if (__any_sync(~0u, some)) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
@@ -500,29 +518,30 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         }
         const float off = (ref == -INFINITY ? 0.f : -ref) + BIAS;
         const uint64_t q2 = pk(qs, qs), off2 = pk(off, off);
-        uint64_t sum = 0, sum1 = 0;
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t p[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int x = 64 * c + 2 * e;
-            const float2 y = un(fma2(pk(__uint_as_float(v[x >> 5][x & 31]), __uint_as_float(v[x >> 5][(x & 31) + 1])), q2, off2));
+            const uint64_t y2 = fma2(pk(__uint_as_float(v[x >> 5][x & 31]), __uint_as_float(v[x >> 5][(x & 31) + 1])), q2, off2);
+            const float2 y = un(y2);
             const float p0 = ex2(y.x), p1 = ex2(y.y);
-            if (e & 1) sum1 = add2(sum1, pk(p0, p1));
-            else sum = add2(sum, pk(p0, p1));
+            sum[e & 3] = add2(sum[e & 3], pk(p0, p1));
             p[e] = Elem<DT>::pack(p0, p1);
           }
           tc5::tmem_st32(ts + 32 * c, p);
+          tc5::tmem_st_wait();
+          tc5::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive(pfull + 16 * i + 8 * c);   // half of P: its products may begin
         }
-        const float2 l2 = un(add2(sum, sum1));
+        const float2 l2 = un(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
         l += l2.x + l2.y;
-        tc5::tmem_st_wait();
-        tc5::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc5::mbar_arrive(pfull + 8 * i);
       }
       if (!run) break;
+      if (l < SEEN) l = 0.f;
       const bool any = t.last >= 0;
       if (any) {
         if (!(run = k16_wait(ofull + 8 * i, oc & 1))) break;
@@ -562,7 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         }
         __stcg(pl + static_cast<long long>(it.slot) * 256 + i * 128 + r, make_float2(ref, l));
         __threadfence();
-        tile_sync(i);
+        if (!(run = tile_sync())) break;
         const int slot0 = it.slot - it.part * it.stride;
         if (r == 0) {
           int* tk = a.tickets + 2 * slot0 + i;
@@ -571,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           flag[i] = old == it.ns - 1;
           __threadfence();
         }
-        tile_sync(i);
+        if (!(run = tile_sync())) break;
         if (flag[i]) {
           const float2* ml = pl + static_cast<long long>(slot0) * 256 + i * 128 + r;
           const float4* pq = reinterpret_cast<const float4*>(a.ws) + static_cast<long long>(slot0) * (2 * (D / 4) * 128) + rr;
@@ -607,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           }
           __syncwarp();
         }
-        tile_sync(i);                                          // (the flag is free again)
+        if (!(run = tile_sync())) break;                       // (the flag is free again)
       }
       tc5::fence_before_sync();
     }
