@@ -1,10 +1,24 @@
-// Eviction from the 16-bit cache: per (row, kv head) the tokens with the largest accumulated attention weight stay.
+// Eviction from the 16-bit cache: per (row, kv head) the tokens with the largest accumulated attention weight stay, in order.
+//
+// HBM bound: 8 D bytes move per kept (token, kv head) (key and value row, read and written), 4 bytes are read per weight.
+// Two launches, the second one's start hidden behind the first (programmatic launch):
+//   k_select  a cluster of 1 to 8 CTAs per (row, kv head): the threshold by a radix search over order-preserving keys (11, 11
+//             and 10 bits; the CTAs' histograms are added through distributed shared memory), then one scan that writes the
+//             kept positions and their weights;
+//   k_copy    (other pages) a CTA per 64 kept tokens, or
+//   k_move    (in place) a cluster per (row, kv head) that moves the rows down step by step: a kept token only moves to a lower
+//             position, so a step's writes hit no row that a later step reads, and one cluster barrier per step is enough.
+#include <cooperative_groups.h>
+
 #include "k16_kernels.h"
+
+namespace cg = cooperative_groups;
 
 namespace k16 {
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 512, NWARP = NT / 32;
+constexpr int BINS = 2048;
 
 // order-preserving key of a weight: a > b as floats iff key(a) > key(b); -0 equals +0, NaN is below everything
 FR_DEVI uint32_t key_of(float w) {
@@ -12,96 +26,272 @@ FR_DEVI uint32_t key_of(float w) {
   const uint32_t u = __float_as_uint(w + 0.f);        // -0 + 0 = +0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-FR_DEVI int block_sum(int v, int* red) {
-  for (int x = 16; x; x >>= 1) v += __shfl_xor_sync(~0u, v, x);
+// exclusive sum over the CTA (every thread's v), and the total
+FR_DEVI unsigned long long block_scan(unsigned long long v, unsigned long long* red, unsigned long long& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  unsigned long long s = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long y = __shfl_up_sync(~0u, s, d);
+    if (lane >= d) s += y;
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if (lane == 31) red[w] = s;
   __syncthreads();
-  int s = 0;
-  for (int i = 0; i < NT / 32; ++i) s += red[i];
-  return s;
+  unsigned long long before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NWARP; ++i) {
+    if (i < w) before += red[i];
+    total += red[i];
+  }
+  return before + s - v;
 }
 
-// CTA per (row, kv head): the threshold key by 32 rounds of bisection on its bits, the kept positions by a scan over
-// the row in order, then the rows in order (in place a step's reads end before its writes begin; a kept row only moves down).
-__global__ void __launch_bounds__(NT) k_evict(EvictArgs a) {
-  __shared__ int red[NT / 32], s_base, s_ties;
-  const int b = blockIdx.x / a.c.Hkv, h = blockIdx.x % a.c.Hkv, tid = threadIdx.x;
+__global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
+  __shared__ uint32_t hist[3][BINS];
+  __shared__ unsigned long long red[NWARP];
+  __shared__ uint32_t s_digit;
+  __shared__ int s_left;
+  __shared__ int s_count[2];                          // this CTA's sure tokens and ties, read by the cluster
+  cg::cluster_group cl = cg::this_cluster();
+  const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x;
+  const int b = g / a.c.Hkv, h = g - b * a.c.Hkv;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const int len = min(a.c.len(b), a.w_len), m = min(len, a.budget);
   const float* w = a.weights + b * a.w_bs + h * a.w_hs;
-  int* kept = a.kept + (static_cast<long long>(b) * a.c.Hkv + h) * a.budget;
-  float* nw = a.new_weights + (static_cast<long long>(b) * a.c.Hkv + h) * a.nw_len;
-  if (h == 0 && tid == 0) a.new_lens[b] = m;
-  if (len <= a.budget) {
-    for (int i = tid; i < len; i += NT) kept[i] = i, nw[i] = w[i];
-  } else {
-    const int lo = a.sinks, hi = len - a.recent, want = a.budget - a.sinks - a.recent;
-    uint32_t T = 0;                                     // the want-th largest key
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t c = T | (1u << bit);
-      int n = 0;
-      for (int i = lo + tid; i < hi; i += NT) n += key_of(w[i]) >= c;
-      if (block_sum(n, red) >= want && want > 0) T = c;
-    }
-    int n = 0;
-    for (int i = lo + tid; i < hi; i += NT) n += key_of(w[i]) > T;
-    const int above = block_sum(n, red);
-    if (tid == 0) s_base = 0, s_ties = want - above;    // ties still to take, lowest position first
+  int* kept = a.kept + static_cast<long long>(g) * a.budget;
+  float* nw = a.new_weights + static_cast<long long>(g) * a.nw_len;
+  if (h == 0 && rank == 0 && tid == 0) a.new_lens[b] = m;
+  for (int i = m + rank * NT + tid; i < a.budget; i += C * NT) kept[i] = -1;
+  for (int i = m + rank * NT + tid; i < a.nw_len; i += C * NT) nw[i] = 0.f;
+  if (len <= a.budget) {                              // (the whole cluster)
+    for (int i = rank * NT + tid; i < len; i += C * NT) kept[i] = i, nw[i] = w[i];
+    return;
+  }
+  const int lo = a.sinks, hi = len - a.recent, want = a.budget - a.sinks - a.recent;   // [lo, hi) is chosen from
+  const int seg = (len + C - 1) / C, s0 = min(rank * seg, len), s1 = min(s0 + seg, len);
+  uint32_t T = 0;                                     // the want-th largest key
+  int left = want;                                    // ... of whose ties this many are taken
+  if (want > 0) {
+    for (int i = tid; i < 3 * BINS; i += NT) (&hist[0][0])[i] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < len; i0 += NT) {
-      const int i = i0 + tid;
-      const bool forced = i < len && (i < lo || i >= hi);
-      const uint32_t k = i < len ? key_of(w[i]) : 0u;
-      const bool tie = i < len && !forced && want > 0 && k == T;
-      bool take = forced || (i < len && !forced && want > 0 && k > T);
-      // exclusive scans over the CTA: ties first, then what is taken
-      __shared__ int wt[NT / 32], wk[NT / 32];
-      const unsigned mt = __ballot_sync(~0u, tie), below = (1u << (tid & 31)) - 1;
-      if ((tid & 31) == 0) wt[tid >> 5] = __popc(mt);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const int sh = p == 0 ? 21 : p == 1 ? 10 : 0, nbits = p == 2 ? 10 : 11;
+      for (int i = max(s0, lo) + tid; i < min(s1, hi); i += NT) {
+        const uint32_t k = key_of(w[i]);
+        if (p == 0 || (k >> (sh + nbits)) == (T >> (sh + nbits))) atomicAdd(&hist[p][(k >> sh) & ((1u << nbits) - 1)], 1u);
+      }
+      cl.sync();
+      // bins from the top, four per thread
+      const int per = BINS / NT, top = (1 << nbits) - 1;
+      int n[per], mine = 0;
+#pragma unroll
+      for (int e = 0; e < per; ++e) {
+        const int q = tid * per + e;
+        n[e] = 0;
+        if (q <= top)
+          for (int r = 0; r < C; ++r) n[e] += static_cast<int>(cl.map_shared_rank(&hist[p][0], r)[top - q]);
+        mine += n[e];
+      }
+      unsigned long long total;
+      int cum = static_cast<int>(block_scan(static_cast<unsigned long long>(mine), red, total));
+#pragma unroll
+      for (int e = 0; e < per; ++e) {
+        if (cum < left && left <= cum + n[e]) {       // one bin of one thread
+          s_digit = static_cast<uint32_t>(top - (tid * per + e));
+          s_left = left - cum;
+        }
+        cum += n[e];
+      }
       __syncthreads();
-      int tb = __popc(mt & below), tt = 0;
-      for (int x = 0; x < NT / 32; ++x) tt += wt[x], tb += x < (tid >> 5) ? wt[x] : 0;
-      take = take || (tie && tb < s_ties);
-      const unsigned mk = __ballot_sync(~0u, take);
-      if ((tid & 31) == 0) wk[tid >> 5] = __popc(mk);
-      __syncthreads();
-      int kb = __popc(mk & below), kt = 0;
-      for (int x = 0; x < NT / 32; ++x) kt += wk[x], kb += x < (tid >> 5) ? wk[x] : 0;
-      if (take) kept[s_base + kb] = i, nw[s_base + kb] = w[i];
-      __syncthreads();
-      if (tid == 0) s_base += kt, s_ties -= min(s_ties, tt);
+      T |= s_digit << sh;
+      left = s_left;
       __syncthreads();
     }
   }
-  for (int i = m + tid; i < a.budget; i += NT) kept[i] = -1;
-  for (int i = m + tid; i < a.nw_len; i += NT) nw[i] = 0.f;
-  if (len <= a.budget && !a.dst_bt) return;
-  __threadfence_block();
+  // every thread a run of positions: sure tokens (forced, or above T) and ties
+  const int run = (seg + NT - 1) / NT, i0 = min(s0 + tid * run, s1), i1 = min(i0 + run, s1);
+  int sure = 0, ties = 0;
+  for (int i = i0; i < i1; ++i) {
+    const bool forced = i < lo || i >= hi;
+    const uint32_t k = key_of(w[i]);
+    sure += forced || (want > 0 && k > T);
+    ties += !forced && want > 0 && k == T;
+  }
+  unsigned long long total;
+  const unsigned long long ex = block_scan((static_cast<unsigned long long>(sure) << 32) | static_cast<unsigned>(ties), red, total);
+  if (tid == 0) s_count[0] = static_cast<int>(total >> 32), s_count[1] = static_cast<int>(total & 0xffffffffu);
+  cl.sync();
+  int pos = 0, tie = 0;                               // kept tokens and ties before this CTA
+  for (int r = 0; r < rank; ++r) {
+    const int* c = cl.map_shared_rank(&s_count[0], r);
+    const int t = c[1];
+    pos += c[0] + min(max(left - tie, 0), t);
+    tie += t;
+  }
+  tie += static_cast<int>(ex & 0xffffffffu);
+  pos += static_cast<int>(ex >> 32) + max(min(tie, left) - min(tie - static_cast<int>(ex & 0xffffffffu), left), 0);
+  for (int i = i0; i < i1; ++i) {
+    const bool forced = i < lo || i >= hi;
+    const float x = w[i];
+    const uint32_t k = key_of(x);
+    bool take = forced || (want > 0 && k > T);
+    if (!forced && want > 0 && k == T) take = tie++ < left;
+    if (take) {
+      kept[pos] = i;
+      nw[pos] = x;
+      ++pos;
+    }
+  }
+  cl.sync();                                          // the others have read this CTA's counts
+}
+
+FR_DEVI void wait_select() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
+// Rows to other pages: a CTA copies TOK kept tokens, 16-byte pieces, eight of each thread's in flight.
+constexpr int CT = 256, TOK = 64;
+template <int D> __global__ void __launch_bounds__(CT) k_copy(EvictArgs a, int chunks) {
+  constexpr int PPR = D / 8, PPT = 2 * PPR;           // pieces per row, per token (key row, then value row)
+  __shared__ long long src[TOK], dst[TOK];            // element offsets of the key rows, or -1 | -2
+  const int g = blockIdx.x / chunks, b = g / a.c.Hkv, h = g - b * a.c.Hkv, r0 = (blockIdx.x - g * chunks) * TOK;
+  wait_select();
+  const int m = a.new_lens[b];
+  if (r0 >= m) return;
+  const int n = min(TOK, m - r0);
+  if (threadIdx.x < TOK) {
+    const int r = r0 + threadIdx.x, t = threadIdx.x;
+    long long s = -1, d = -1;
+    if (t < n) {
+      const int j = a.kept[static_cast<long long>(g) * a.budget + r], ps = a.c.page_of(b, j);
+      const int pd = a.dst_bt[b * a.dst_stride + (r >> a.c.page_sh)];
+      if (ps >= 0) s = row_at(ps, a.c.Hkv, h, 0, a.c.page_sh, j & (a.c.page() - 1), D);
+      if (pd >= 0 && pd < a.dst_pages) d = row_at(pd, a.c.Hkv, h, 0, a.c.page_sh, r & (a.c.page() - 1), D);
+    }
+    src[t] = s;
+    dst[t] = d;
+  }
   __syncthreads();
-  // rows: 16-byte pieces, NT at a time; a step covers whole tokens (D / 4 pieces: key row, then value row)
-  const int ppt = a.D >> 2, tps = NT / ppt;
-  for (int r0 = 0; r0 < m; r0 += tps) {
-    const int r = r0 + tid / ppt, piece = tid % ppt, kv = piece >= ppt / 2, e = (piece - kv * (ppt / 2)) * 8;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < m) {
-      const int src = kept[r], pg = a.c.page_of(b, src);
-      if (pg >= 0) x = *reinterpret_cast<const uint4*>(a.c.pool + row_at(pg, a.c.Hkv, h, kv, a.c.page_sh, src & (a.c.page() - 1), a.D) + e);
-    }
-    __syncthreads();
-    if (r < m) {
-      const int pg = a.dst_bt ? a.dst_bt[b * a.dst_stride + (r >> a.c.page_sh)] : a.c.page_of(b, r);
-      if (pg >= 0 && pg < a.dst_pages)
-        *reinterpret_cast<uint4*>(a.dst + row_at(pg, a.c.Hkv, h, kv, a.c.page_sh, r & (a.c.page() - 1), a.D) + e) = x;
-    }
-    __syncthreads();
+  const long long v = static_cast<long long>(D) << a.c.page_sh;   // from a key row to its value row
+  constexpr int IT = TOK * PPT / CT;
+  uint4 x[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int p = i * CT + threadIdx.x, t = p / PPT, e = p % PPT;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (src[t] >= 0) x[i] = __ldcs(reinterpret_cast<const uint4*>(a.c.pool + src[t] + (e / PPR) * v + (e % PPR) * 8));
   }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int p = i * CT + threadIdx.x, t = p / PPT, e = p % PPT;
+    if (dst[t] >= 0) *reinterpret_cast<uint4*>(a.dst + dst[t] + (e / PPR) * v + (e % PPR) * 8) = x[i];
+  }
+}
+
+// In place: step s moves the kept tokens [s C R, (s + 1) C R).  A step's sources are read into registers before the barrier
+// behind which it writes, while the step before it writes: those writes end below every position that is being read.
+template <int D> __global__ void __launch_bounds__(NT) k_move(EvictArgs a, int C) {
+  constexpr int PPR = D / 8, PPT = 2 * PPR, IT = 8, R = IT * NT / PPT;   // tokens per CTA and step
+  cg::cluster_group cl = cg::this_cluster();
+  const int g = blockIdx.x / C, rank = blockIdx.x - g * C, b = g / a.c.Hkv, h = g - b * a.c.Hkv;
+  wait_select();
+  const int len = min(a.c.len(b), a.w_len), m = a.new_lens[b];
+  if (len <= a.budget) return;                        // (the whole cluster)
+  const int* kept = a.kept + static_cast<long long>(g) * a.budget;
+  uint16_t* pool = a.dst;
+  const int steps = (m + C * R - 1) / (C * R);
+  const auto row = [&](int j) -> long long {
+    const int pg = a.c.page_of(b, j);
+    return pg < 0 ? -1 : row_at(pg, a.c.Hkv, h, 0, a.c.page_sh, j & (a.c.page() - 1), D);
+  };
+  const long long v = static_cast<long long>(D) << a.c.page_sh;
+  const int e = threadIdx.x % PPT, t0 = threadIdx.x / PPT;
+  const long long eo = (e / PPR) * v + (e % PPR) * 8;
+  uint4 x[IT];
+  bool moved[IT];
+  const auto read = [&](int s, uint4 (&y)[IT], bool (&mv)[IT]) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = (s * C + rank) * R + i * (NT / PPT) + t0;
+      mv[i] = false;
+      y[i] = make_uint4(0, 0, 0, 0);
+      if (r < m) {
+        const int j = kept[r];
+        mv[i] = j != r;
+        if (j != r) {
+          const long long o = row(j);
+          if (o >= 0) y[i] = __ldcg(reinterpret_cast<const uint4*>(pool + o + eo));
+        }
+      }
+    }
+  };
+  read(0, x, moved);
+  for (int s = 0; s < steps; ++s) {
+    cl.sync();                                        // every source of this step is in registers
+    uint4 y[IT];
+    bool my[IT];
+    if (s + 1 < steps) read(s + 1, y, my);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = (s * C + rank) * R + i * (NT / PPT) + t0;
+      if (moved[i]) {
+        const long long o = row(r);
+        if (o >= 0) __stcg(reinterpret_cast<uint4*>(pool + o + eo), x[i]);
+      }
+    }
+    if (s + 1 < steps)
+#pragma unroll
+      for (int i = 0; i < IT; ++i) x[i] = y[i], moved[i] = my[i];
+  }
+}
+
+template <class... Ts>
+cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, int cluster, bool dependent, cudaStream_t st, Ts... args) {
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.stream = st;
+  c.attrs = at;
+  if (cluster > 0) {
+    at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[c.numAttrs].val.clusterDim.x = cluster;
+    at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
+    ++c.numAttrs;
+  }
+  if (dependent) {
+    at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++c.numAttrs;
+  }
+  return cudaLaunchKernelEx(&c, k, args...);
+}
+
+// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each
+int cluster_of(long long groups, long long positions) {
+  int c = 1;
+  while (c < 8 && groups * c < 148 && positions / c > 2048) c *= 2;
+  return c;
 }
 
 }  // namespace
 
 cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
-  k_evict<<<a.B * a.c.Hkv, NT, 0, st>>>(a);
-  return cudaGetLastError();
+  const long long groups = static_cast<long long>(a.B) * a.c.Hkv;
+  const long long width = static_cast<long long>(a.c.bt_width) << a.c.page_sh;
+  const int c = cluster_of(groups, width < a.w_len ? width : a.w_len);
+  if (cudaError_t e = launch(k_select, static_cast<unsigned>(groups * c), NT, c, false, st, a, c)) return e;
+  if (!a.dst_bt) {
+    const int cm = cluster_of(groups, a.budget);
+    return a.D == 128 ? launch(k_move<128>, static_cast<unsigned>(groups * cm), NT, cm, true, st, a, cm)
+                      : launch(k_move<64>, static_cast<unsigned>(groups * cm), NT, cm, true, st, a, cm);
+  }
+  const long long longest = width < a.budget ? width : a.budget, chunks = (longest + TOK - 1) / TOK;
+  if (chunks == 0) return cudaSuccess;
+  if (chunks * groups > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  return a.D == 128 ? launch(k_copy<128>, static_cast<unsigned>(groups * chunks), CT, 0, true, st, a, static_cast<int>(chunks))
+                    : launch(k_copy<64>, static_cast<unsigned>(groups * chunks), CT, 0, true, st, a, static_cast<int>(chunks));
 }
 
 }  // namespace k16

@@ -1,32 +1,48 @@
-// Row writer of the 16-bit cache: a copy of 16-byte pieces from the projection's output to the pages.
+// Row writer of the 16-bit cache: a copy of 16-byte pieces from the projection's output to the pages.  HBM bound (every byte is
+// read once and written once); a decode step's few rows are bound by the launch.
 #include "k16_kernels.h"
 
 namespace k16 {
 namespace {
 
-// One thread per 16-byte piece.
-__global__ void k_write(const uint16_t* __restrict__ kv, long long kv_ts, long long kv_hs, const long long* __restrict__ slots, int T,
-                        int Hkv, int D, int page_sh, long long nslots, uint16_t* __restrict__ pool) {
-  const int ppr = D >> 3, ppt = 2 * Hkv * ppr;          // pieces per row, per token
-  const long long i = blockIdx.x * 256ll + threadIdx.x;
-  const long long t = i / ppt;
-  if (t >= T) return;
-  const int r = static_cast<int>(i - t * ppt), row = r / ppr, piece = r - row * ppr;
-  const long long s = slots[t];
-  if (s < 0 || s >= nslots) return;
-  const int h = row < Hkv ? row : row - Hkv;
-  const uint4 x = *reinterpret_cast<const uint4*>(kv + t * kv_ts + row * kv_hs + piece * 8);
-  *reinterpret_cast<uint4*>(pool + row_at(s >> page_sh, Hkv, h, row >= Hkv, page_sh, static_cast<int>(s & ((1 << page_sh) - 1)), D) +
-                            piece * 8) = x;
+// A CTA copies PER * CT consecutive pieces (piece = token, row, 16 bytes of it), PER of them in flight per thread.
+constexpr int CT = 256;
+template <int PER>
+__global__ void __launch_bounds__(CT) k_write(const uint16_t* __restrict__ kv, long long kv_ts, long long kv_hs,
+                                              const long long* __restrict__ slots, int T, int Hkv, int D, int page_sh, long long nslots,
+                                              uint16_t* __restrict__ pool) {
+  const int psh = D == 128 ? 4 : 3, ppt = 2 * Hkv << psh;      // pieces per row (log2), per token
+  const long long first = static_cast<long long>(blockIdx.x) * (PER * CT);
+  const int tok0 = static_cast<int>(first / ppt);
+  const unsigned rem = static_cast<unsigned>(first - static_cast<long long>(tok0) * ppt) + threadIdx.x;
+  uint4 x[PER];
+  uint16_t* to[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const unsigned p = rem + i * CT, dt = p / ppt, r = p - dt * ppt;
+    const int t = tok0 + static_cast<int>(dt), row = static_cast<int>(r >> psh), piece = static_cast<int>(r & ((1 << psh) - 1));
+    to[i] = nullptr;
+    if (t >= T) continue;
+    const long long s = slots[t];
+    if (s < 0 || s >= nslots) continue;
+    const int h = row < Hkv ? row : row - Hkv;
+    to[i] = pool + row_at(s >> page_sh, Hkv, h, row >= Hkv, page_sh, static_cast<int>(s & ((1 << page_sh) - 1)), D) + piece * 8;
+    x[i] = __ldcs(reinterpret_cast<const uint4*>(kv + t * kv_ts + row * kv_hs + piece * 8));
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (to[i]) *reinterpret_cast<uint4*>(to[i]) = x[i];
 }
 
 }  // namespace
 
 cudaError_t write_rows(const uint16_t* kv, long long kv_ts, long long kv_hs, const long long* slots, int T, int Hkv, int D,
                        int page_sh, long long num_pages, uint16_t* pool, cudaStream_t st) {
-  const long long n = static_cast<long long>(T) * 2 * Hkv * (D >> 3);
-  k_write<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(kv, kv_ts, kv_hs, slots, T, Hkv, D, page_sh, num_pages << page_sh,
-                                                                  pool);
+  const long long n = static_cast<long long>(T) * 2 * Hkv * (D >> 3), nslots = num_pages << page_sh;
+  if (n > 148ll * 8 * 4 * CT)          // more than one piece for every thread the SMs hold: four in flight per thread
+    k_write<4><<<static_cast<unsigned>((n + 4 * CT - 1) / (4 * CT)), CT, 0, st>>>(kv, kv_ts, kv_hs, slots, T, Hkv, D, page_sh, nslots, pool);
+  else
+    k_write<1><<<static_cast<unsigned>((n + CT - 1) / CT), CT, 0, st>>>(kv, kv_ts, kv_hs, slots, T, Hkv, D, page_sh, nslots, pool);
   return cudaGetLastError();
 }
 
