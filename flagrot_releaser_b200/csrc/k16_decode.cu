@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
     *abort = 0;
     tma_prefetch_map(&map);
   }
+  if (scores) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   // the list's length; rows that see nothing are written as zeros here
   long long total = 0;
   for (int b = tid; b < a.B; b += THREADS) {
@@ -418,36 +419,56 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
   }
 }
 
-// weights[b, h, j] += sum over the head group of 2^(score - lse), a thread per key
-__global__ void __launch_bounds__(256) k_weights(AttnArgs a, const float* scores, long long score_ld, const float* lse, int chunks) {
+// weights[b, h, j] += sum over the head group of 2^(score - lse): four keys per thread; VEC: the weights' rows are 16-byte
+// aligned.  Launched behind k_decode's start (programmatic launch).
+template <bool VEC> __global__ void __launch_bounds__(256) k_weights(AttnArgs a, const float* scores, long long score_ld, const float* lse, int chunks) {
   const int bh = blockIdx.x / chunks, b = bh / a.c.Hkv, h = bh - b * a.c.Hkv, Hq = a.c.Hkv * a.G;
-  const int len = a.c.len(b), j = (blockIdx.x - bh * chunks) * 256 + threadIdx.x;
+  const int len = a.c.len(b), j = (blockIdx.x - bh * chunks) * 1024 + 4 * threadIdx.x;
   const Span sp(len - 1, a.window, a.sinks);
-  if (j >= len || (j >= sp.s1 && j < sp.lo)) return;
-  float w = 0.f;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (j >= len || (j >= sp.s1 && j + 4 <= sp.lo)) return;
+  float* w = a.weights + b * a.w_bs + h * a.w_hs + j;
+  const bool all = j + 4 <= len && (j >= sp.lo || j + 4 <= sp.s1);
+  float4 old;
+  if (VEC && all) old = *reinterpret_cast<const float4*>(w);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  const long long r0 = static_cast<long long>(b) * Hq + h * a.G;
+#pragma unroll 4
   for (int g = 0; g < a.G; ++g) {
-    const long long r = static_cast<long long>(b) * Hq + h * a.G + g;
-    w += ex2(scores[r * score_ld + j] - lse[r]);
+    const float4 s = __ldcs(reinterpret_cast<const float4*>(scores + (r0 + g) * score_ld + j));
+    const float m = lse[r0 + g];
+    x.x += ex2(s.x - m);
+    x.y += ex2(s.y - m);
+    x.z += ex2(s.z - m);
+    x.w += ex2(s.w - m);
   }
-  a.weights[b * a.w_bs + h * a.w_hs + j] += w;
+  if (VEC && all) {
+    *reinterpret_cast<float4*>(w) = make_float4(old.x + x.x, old.y + x.y, old.z + x.z, old.w + x.w);
+  } else {
+    const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < len && (j + e < sp.s1 || j + e >= sp.lo)) w[e] += y[e];
+  }
 }
 
 long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
 template <int DT, int D, int NT>
-cudaError_t launch(const AttnArgs& a, const CUtensorMap& map, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
+cudaError_t launch(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                    cudaStream_t st) {
   const auto k = k_decode<DT, D, NT>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return e;
+  static std::atomic<bool> done[MAX_DEVICES];
+  if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
   k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, map, nhg, part, lse, scores, ld);
   return cudaGetLastError();
 }
 template <int DT, int D>
-cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
+cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                       cudaStream_t st) {
-  if (a.G <= 8) return launch<DT, D, 1>(a, map, grid, nhg, part, lse, scores, ld, st);
-  if (a.G <= 16) return launch<DT, D, 2>(a, map, grid, nhg, part, lse, scores, ld, st);
-  return launch<DT, D, 4>(a, map, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 8) return launch<DT, D, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 16) return launch<DT, D, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  return launch<DT, D, 4>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
 }
 
 }  // namespace
@@ -466,8 +487,7 @@ int decode_status() {
 
 cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st) {
   int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaError_t e = device_sms(dev, sms);
   if (e != cudaSuccess) return e;
   CUtensorMap map;
   e = pool_map(&map, dtype, a.c.pool, (a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh, a.D, 32);
@@ -479,14 +499,24 @@ cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st) {
   float* scores = a.weights ? lse + up(R * 4, 256) / 4 : nullptr;
   const int nhg = (a.G + MAX_GT - 1) / MAX_GT, grid = 2 * sms < MAX_CTAS ? 2 * sms : MAX_CTAS;
   if (dtype == 0)
-    e = a.D == 128 ? launch_nt<0, 128>(a, map, grid, nhg, part, lse, scores, ld, st) : launch_nt<0, 64>(a, map, grid, nhg, part, lse, scores, ld, st);
+    e = a.D == 128 ? launch_nt<0, 128>(a, map, dev, grid, nhg, part, lse, scores, ld, st) : launch_nt<0, 64>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
   else
-    e = a.D == 128 ? launch_nt<1, 128>(a, map, grid, nhg, part, lse, scores, ld, st) : launch_nt<1, 64>(a, map, grid, nhg, part, lse, scores, ld, st);
+    e = a.D == 128 ? launch_nt<1, 128>(a, map, dev, grid, nhg, part, lse, scores, ld, st) : launch_nt<1, 64>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
   if (e != cudaSuccess || !a.weights || width == 0) return e;
-  const long long chunks = (width + 255) / 256;
+  const long long chunks = (width + 1023) / 1024;
   if (chunks * a.B * a.c.Hkv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  k_weights<<<static_cast<unsigned>(chunks * a.B * a.c.Hkv), 256, 0, st>>>(a, scores, ld, lse, static_cast<int>(chunks));
-  return cudaGetLastError();
+  const bool vec = (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0 && a.w_bs % 4 == 0 && a.w_hs % 4 == 0;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(static_cast<unsigned>(chunks * a.B * a.c.Hkv));
+  c.blockDim = dim3(256);
+  c.stream = st;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, vec ? k_weights<true> : k_weights<false>, a, static_cast<const float*>(scores), ld,
+                            static_cast<const float*>(lse), static_cast<int>(chunks));
 }
 
 }  // namespace k16

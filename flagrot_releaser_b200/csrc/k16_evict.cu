@@ -11,6 +11,7 @@
 #include <cooperative_groups.h>
 
 #include "k16_kernels.h"
+#include "k16_tma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -19,6 +20,7 @@ namespace {
 
 constexpr int NT = 512, NWARP = NT / 32;
 constexpr int BINS = 2048;
+constexpr int MAX_KEYS = 16384;                       // keys of a CTA's positions that shared memory holds
 
 // order-preserving key of a weight: a > b as floats iff key(a) > key(b); -0 equals +0, NaN is below everything
 FR_DEVI uint32_t key_of(float w) {
@@ -26,42 +28,57 @@ FR_DEVI uint32_t key_of(float w) {
   const uint32_t u = __float_as_uint(w + 0.f);        // -0 + 0 = +0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-// exclusive sum over the CTA (every thread's v), and the total
-FR_DEVI unsigned long long block_scan(unsigned long long v, unsigned long long* red, unsigned long long& total) {
+// exclusive sum over the CTA
+FR_DEVI int block_scan(int v, int* red) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  unsigned long long s = v;
+  int s = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long y = __shfl_up_sync(~0u, s, d);
+    const int y = __shfl_up_sync(~0u, s, d);
     if (lane >= d) s += y;
   }
   __syncthreads();
   if (lane == 31) red[w] = s;
   __syncthreads();
-  unsigned long long before = 0;
-  total = 0;
+  int before = 0;
 #pragma unroll
-  for (int i = 0; i < NWARP; ++i) {
+  for (int i = 0; i < NWARP; ++i)
     if (i < w) before += red[i];
-    total += red[i];
-  }
   return before + s - v;
 }
 
-__global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
-  __shared__ uint32_t hist[3][BINS];
-  __shared__ unsigned long long red[NWARP];
+// STAGED: the CTA's weights are read once and kept in shared memory (at most MAX_KEYS); else every pass reads them again.
+// CL: the cluster has more than one CTA.
+template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
+  extern __shared__ float sw[];
+  __shared__ int hist[3][BINS];
+  __shared__ int red[NWARP], s_sure[NWARP], s_ties[NWARP], s_slice[3];
   __shared__ uint32_t s_digit;
   __shared__ int s_left;
   __shared__ int s_count[2];                          // this CTA's sure tokens and ties, read by the cluster
   cg::cluster_group cl = cg::this_cluster();
-  const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x;
+  const auto sync = [&]() {
+    if (CL) cl.sync();
+    else __syncthreads();
+  };
+  const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int b = g / a.c.Hkv, h = g - b * a.c.Hkv;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const int len = min(a.c.len(b), a.w_len), m = min(len, a.budget);
   const float* w = a.weights + b * a.w_bs + h * a.w_hs;
   int* kept = a.kept + static_cast<long long>(g) * a.budget;
   float* nw = a.new_weights + static_cast<long long>(g) * a.nw_len;
+  const int seg = (len + C - 1) / C, s0 = min(rank * seg, len), s1 = min(s0 + seg, len);
+  if (STAGED && len > a.budget) {                     // eight loads of a thread in flight
+    for (int i = s0 + tid; i < s1; i += 8 * NT) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = i + e * NT < s1 ? w[i + e * NT] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e * NT < s1) sw[i + e * NT - s0] = x[e];
+    }
+  }
   if (h == 0 && rank == 0 && tid == 0) a.new_lens[b] = m;
   for (int i = m + rank * NT + tid; i < a.budget; i += C * NT) kept[i] = -1;
   for (int i = m + rank * NT + tid; i < a.nw_len; i += C * NT) nw[i] = 0.f;
@@ -70,37 +87,71 @@ __global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
     return;
   }
   const int lo = a.sinks, hi = len - a.recent, want = a.budget - a.sinks - a.recent;   // [lo, hi) is chosen from
-  const int seg = (len + C - 1) / C, s0 = min(rank * seg, len), s1 = min(s0 + seg, len);
+  const auto weight = [&](int i) { return STAGED ? sw[i - s0] : w[i]; };
   uint32_t T = 0;                                     // the want-th largest key
   int left = want;                                    // ... of whose ties this many are taken
+  for (int i = tid; i < 3 * BINS; i += NT) (&hist[0][0])[i] = 0;
+  __syncthreads();
   if (want > 0) {
-    for (int i = tid; i < 3 * BINS; i += NT) (&hist[0][0])[i] = 0;
-    __syncthreads();
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      const int sh = p == 0 ? 21 : p == 1 ? 10 : 0, nbits = p == 2 ? 10 : 11;
+      const int sh = p == 0 ? 21 : p == 1 ? 10 : 0, nbits = p == 2 ? 10 : 11, bins = 1 << nbits;
       for (int i = max(s0, lo) + tid; i < min(s1, hi); i += NT) {
-        const uint32_t k = key_of(w[i]);
-        if (p == 0 || (k >> (sh + nbits)) == (T >> (sh + nbits))) atomicAdd(&hist[p][(k >> sh) & ((1u << nbits) - 1)], 1u);
+        const uint32_t k = key_of(weight(i));
+        if (p == 0 || (k >> (sh + nbits)) == (T >> (sh + nbits))) atomicAdd(&hist[p][(k >> sh) & (bins - 1)], 1);
       }
-      cl.sync();
-      // bins from the top, four per thread
-      const int per = BINS / NT, top = (1 << nbits) - 1;
+      sync();
+      // Counts from the top bin down.  A cluster adds its histograms slice by slice: CTA r the slice of bins/C bins that is
+      // r-th from the top, in place (only r reads or writes it from then on, until the others look the slice of the answer up).
+      int first = 0, width = bins, owner = rank, before = 0;   // slice: bins [top - first - width + 1, top - first]
+      const int top = bins - 1;
+      if (CL) {
+        width = bins / C;
+        first = rank * width;
+        int sum = 0;
+        for (int q = tid; q < width; q += NT) {
+          int n[8], t = 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) n[r] = r < C ? cl.map_shared_rank(&hist[p][0], r)[top - first - q] : 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) t += n[r];
+          hist[p][top - first - q] = t;
+          sum += t;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane == 0) red[wid] = sum;
+        __syncthreads();
+        if (tid == 0) {
+          int t = 0;
+          for (int i = 0; i < NWARP; ++i) t += red[i];
+          s_slice[p] = t;
+        }
+        sync();
+        owner = 0;
+        int n[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) n[r] = r < C ? *cl.map_shared_rank(&s_slice[p], r) : 0;
+#pragma unroll
+        for (int r = 0; r < 7; ++r)
+          if (owner == r && before + n[r] < left) before += n[r], owner = r + 1;
+        first = owner * width;
+      }
+      // the bin of the slice in which the count reaches `left`
+      const int per = BINS / NT;
+      const int* hs = CL ? cl.map_shared_rank(&hist[p][0], owner) : &hist[p][0];
       int n[per], mine = 0;
 #pragma unroll
       for (int e = 0; e < per; ++e) {
         const int q = tid * per + e;
-        n[e] = 0;
-        if (q <= top)
-          for (int r = 0; r < C; ++r) n[e] += static_cast<int>(cl.map_shared_rank(&hist[p][0], r)[top - q]);
+        n[e] = q < width ? hs[top - first - q] : 0;
         mine += n[e];
       }
-      unsigned long long total;
-      int cum = static_cast<int>(block_scan(static_cast<unsigned long long>(mine), red, total));
+      int cum = before + block_scan(mine, red);
 #pragma unroll
       for (int e = 0; e < per; ++e) {
         if (cum < left && left <= cum + n[e]) {       // one bin of one thread
-          s_digit = static_cast<uint32_t>(top - (tid * per + e));
+          s_digit = static_cast<uint32_t>(top - first - (tid * per + e));
           s_left = left - cum;
         }
         cum += n[e];
@@ -111,41 +162,60 @@ __global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
       __syncthreads();
     }
   }
-  // every thread a run of positions: sure tokens (forced, or above T) and ties
-  const int run = (seg + NT - 1) / NT, i0 = min(s0 + tid * run, s1), i1 = min(i0 + run, s1);
+  // a warp's positions are consecutive: sure tokens (forced, or above T) and ties are counted, then written, 32 at a time
+  const int wseg = ((seg + NWARP - 1) / NWARP + 31) & ~31, i0 = min(s0 + wid * wseg, s1), i1 = min(i0 + wseg, s1);
+  const auto kind = [&](int i, bool& tie) {           // sure to be kept; or a tie
+    if (i < lo || i >= hi) return i < i1;
+    const uint32_t k = i < i1 ? key_of(weight(i)) : 0u;
+    tie = i < i1 && want > 0 && k == T;
+    return i < i1 && want > 0 && k > T;
+  };
   int sure = 0, ties = 0;
-  for (int i = i0; i < i1; ++i) {
-    const bool forced = i < lo || i >= hi;
-    const uint32_t k = key_of(w[i]);
-    sure += forced || (want > 0 && k > T);
-    ties += !forced && want > 0 && k == T;
+  for (int i = i0; i < i1; i += 32) {
+    bool tie = false;
+    const bool s = kind(i + lane, tie);
+    sure += __popc(__ballot_sync(~0u, s));
+    ties += __popc(__ballot_sync(~0u, tie));
   }
-  unsigned long long total;
-  const unsigned long long ex = block_scan((static_cast<unsigned long long>(sure) << 32) | static_cast<unsigned>(ties), red, total);
-  if (tid == 0) s_count[0] = static_cast<int>(total >> 32), s_count[1] = static_cast<int>(total & 0xffffffffu);
-  cl.sync();
-  int pos = 0, tie = 0;                               // kept tokens and ties before this CTA
-  for (int r = 0; r < rank; ++r) {
-    const int* c = cl.map_shared_rank(&s_count[0], r);
-    const int t = c[1];
-    pos += c[0] + min(max(left - tie, 0), t);
-    tie += t;
+  if (lane == 0) s_sure[wid] = sure, s_ties[wid] = ties;
+  __syncthreads();
+  int pos = 0, tie0 = 0;                              // this CTA's before this warp
+  sure = ties = 0;
+#pragma unroll
+  for (int i = 0; i < NWARP; ++i) {
+    if (i == wid) pos = sure, tie0 = ties;
+    sure += s_sure[i];
+    ties += s_ties[i];
   }
-  tie += static_cast<int>(ex & 0xffffffffu);
-  pos += static_cast<int>(ex >> 32) + max(min(tie, left) - min(tie - static_cast<int>(ex & 0xffffffffu), left), 0);
-  for (int i = i0; i < i1; ++i) {
-    const bool forced = i < lo || i >= hi;
-    const float x = w[i];
-    const uint32_t k = key_of(x);
-    bool take = forced || (want > 0 && k > T);
-    if (!forced && want > 0 && k == T) take = tie++ < left;
-    if (take) {
-      kept[pos] = i;
-      nw[pos] = x;
-      ++pos;
+  int cta_tie = 0, cta_pos = 0;                       // ties and kept tokens before this CTA
+  if (CL) {
+    if (tid == 0) s_count[0] = sure, s_count[1] = ties;
+    sync();
+    for (int r = 0; r < rank; ++r) {
+      const int* c = cl.map_shared_rank(&s_count[0], r);
+      const int t = c[1];
+      cta_pos += c[0] + min(max(left - cta_tie, 0), t);
+      cta_tie += t;
     }
   }
-  cl.sync();                                          // the others have read this CTA's counts
+  int tie_at = cta_tie + tie0;
+  pos += cta_pos + min(tie_at, left) - min(cta_tie, left);
+  const unsigned below = (1u << lane) - 1;
+  for (int i = i0; i < i1; i += 32) {
+    bool tie = false;
+    bool take = kind(i + lane, tie);
+    const unsigned mt = __ballot_sync(~0u, tie);
+    if (tie) take = tie_at + __popc(mt & below) < left;
+    const unsigned mk = __ballot_sync(~0u, take);
+    if (take) {
+      const int at = pos + __popc(mk & below);
+      kept[at] = i + lane;
+      nw[at] = weight(i + lane);
+    }
+    tie_at += __popc(mt);
+    pos += __popc(mk);
+  }
+  if (CL) sync();                                     // the others have read this CTA's counts
 }
 
 FR_DEVI void wait_select() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
@@ -247,12 +317,14 @@ template <int D> __global__ void __launch_bounds__(NT) k_move(EvictArgs a, int C
 }
 
 template <class... Ts>
-cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, int cluster, bool dependent, cudaStream_t st, Ts... args) {
+cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, size_t smem, int cluster, bool dependent, cudaStream_t st,
+                   Ts... args) {
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(grid);
   c.blockDim = dim3(threads);
   c.stream = st;
+  c.dynamicSmemBytes = smem;
   c.attrs = at;
   if (cluster > 0) {
     at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
@@ -268,10 +340,10 @@ cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, int cluste
   return cudaLaunchKernelEx(&c, k, args...);
 }
 
-// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each
+// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each, and to hold the keys in shared memory
 int cluster_of(long long groups, long long positions) {
   int c = 1;
-  while (c < 8 && groups * c < 148 && positions / c > 2048) c *= 2;
+  while (c < 8 && ((groups * c < 148 && positions / c > 2048) || positions / c > MAX_KEYS)) c *= 2;
   return c;
 }
 
@@ -280,18 +352,30 @@ int cluster_of(long long groups, long long positions) {
 cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
   const long long groups = static_cast<long long>(a.B) * a.c.Hkv;
   const long long width = static_cast<long long>(a.c.bt_width) << a.c.page_sh;
-  const int c = cluster_of(groups, width < a.w_len ? width : a.w_len);
-  if (cudaError_t e = launch(k_select, static_cast<unsigned>(groups * c), NT, c, false, st, a, c)) return e;
+  const long long most = width < a.w_len ? width : a.w_len;
+  const int c = cluster_of(groups, most);
+  const long long seg = (most + c - 1) / c;
+  cudaError_t e;
+  if (seg <= MAX_KEYS) {
+    const auto k = c > 1 ? k_select<true, true> : k_select<true, false>;
+    static std::atomic<bool> done[2][MAX_DEVICES];
+    int dev = 0, sms = 0;
+    if ((e = device_sms(dev, sms)) || (e = allow_smem(k, MAX_KEYS * 4, dev, done[c > 1]))) return e;
+    e = launch(k, static_cast<unsigned>(groups * c), NT, static_cast<size_t>(seg) * 4, c, false, st, a, c);
+  } else {                                            // (the largest cluster)
+    e = launch(k_select<false, true>, static_cast<unsigned>(groups * c), NT, 0, c, false, st, a, c);
+  }
+  if (e != cudaSuccess) return e;
   if (!a.dst_bt) {
     const int cm = cluster_of(groups, a.budget);
-    return a.D == 128 ? launch(k_move<128>, static_cast<unsigned>(groups * cm), NT, cm, true, st, a, cm)
-                      : launch(k_move<64>, static_cast<unsigned>(groups * cm), NT, cm, true, st, a, cm);
+    return a.D == 128 ? launch(k_move<128>, static_cast<unsigned>(groups * cm), NT, 0, cm, true, st, a, cm)
+                      : launch(k_move<64>, static_cast<unsigned>(groups * cm), NT, 0, cm, true, st, a, cm);
   }
   const long long longest = width < a.budget ? width : a.budget, chunks = (longest + TOK - 1) / TOK;
   if (chunks == 0) return cudaSuccess;
   if (chunks * groups > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  return a.D == 128 ? launch(k_copy<128>, static_cast<unsigned>(groups * chunks), CT, 0, true, st, a, static_cast<int>(chunks))
-                    : launch(k_copy<64>, static_cast<unsigned>(groups * chunks), CT, 0, true, st, a, static_cast<int>(chunks));
+  return a.D == 128 ? launch(k_copy<128>, static_cast<unsigned>(groups * chunks), CT, 0, 0, true, st, a, static_cast<int>(chunks))
+                    : launch(k_copy<64>, static_cast<unsigned>(groups * chunks), CT, 0, 0, true, st, a, static_cast<int>(chunks));
 }
 
 }  // namespace k16

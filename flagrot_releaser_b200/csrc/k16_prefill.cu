@@ -640,9 +640,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 }
 
 template <int DT, int D>
-cudaError_t launch(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int grid, cudaStream_t st) {
+cudaError_t launch(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int dev, int grid, cudaStream_t st) {
   const auto k = k_prefill<DT, D>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return e;
+  static std::atomic<bool> done[MAX_DEVICES];
+  if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
   k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, qm, kv, hb, nhg, box);
   return cudaGetLastError();
 }
@@ -671,8 +672,7 @@ int prefill_status() {
 
 cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
   int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaError_t e = device_sms(dev, sms);
   if (e != cudaSuccess) return e;
   int nhg, hb, tpt;
   groups(a.G, nhg, hb, tpt);
@@ -686,8 +686,8 @@ cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
   const long long items = max_pairs(a.B, a.c.Hkv, a.G, a.T) * MAX_SPLIT;
   const int grid = static_cast<int>(items < sms ? items : sms);
   if (dtype == 0)
-    return a.D == 128 ? launch<0, 128>(a, qm, kv, hb, nhg, box, grid, st) : launch<0, 64>(a, qm, kv, hb, nhg, box, grid, st);
-  return a.D == 128 ? launch<1, 128>(a, qm, kv, hb, nhg, box, grid, st) : launch<1, 64>(a, qm, kv, hb, nhg, box, grid, st);
+    return a.D == 128 ? launch<0, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch<0, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
+  return a.D == 128 ? launch<1, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch<1, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
 }
 
 }  // namespace k16

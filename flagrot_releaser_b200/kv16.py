@@ -70,15 +70,12 @@ def _check(rc, what):
         raise RuntimeError(f"{what}: failed (code {rc}, {lib().k16_last_error().decode()})")
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
-
-
-def _here(*tensors):
-    """every tensor is on the current device, to whose current stream the launch goes"""
+def _stream(*tensors):
+    """the current stream of the current device, on which every tensor has to be"""
     dev = torch.cuda.current_device()
     for t in tensors:
         assert t.get_device() == dev, f"tensor on {t.device}, current device cuda:{dev}"
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def chunk_bytes(page: int, D: int = 128) -> int:
@@ -103,96 +100,99 @@ class Workspace:
         self.ntickets = int(L.k16_ws_tickets(rows, Hkv, G, new_tokens))
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
         self.tickets = torch.zeros(max(self.ntickets, 1), dtype=torch.int32, device=device)
+        self.pbuf, self.ptickets = self.buf.data_ptr(), self.tickets.data_ptr()
 
 
 def _pool_ok(pool):
-    assert pool.dim() == 5 and pool.shape[2] == 2 and pool.dtype in DTYPES and pool.is_contiguous(), \
-        "pool: [num_pages, Hkv, 2, page, D] bf16 | fp16, contiguous"
-    assert pool.shape[3] in PAGES and pool.shape[4] in HEAD_DIMS, "page 16 | 32 | 64 | 128, head dim 64 | 128"
+    """(num_pages, Hkv, page, D)"""
+    assert pool.dim() == 5 and pool.dtype in DTYPES and pool.is_contiguous(), "pool: [num_pages, Hkv, 2, page, D] bf16 | fp16, contiguous"
+    npg, Hkv, two, page, D = pool.shape
+    assert two == 2 and page in PAGES and D in HEAD_DIMS, "page 16 | 32 | 64 | 128, head dim 64 | 128"
+    return npg, Hkv, page, D
 
 
 def _table_ok(block_table, B):
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B
-    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1
+    """(width, row stride)"""
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2
+    rows, width = block_table.shape
+    st = block_table.stride()
+    assert rows == B and (st[1] == 1 or width <= 1), "block_table: int32 [B, width]"
+    return width, st[0]
 
 
 def _lens_ok(lens, B):
-    assert lens.dtype == torch.int32 and lens.shape == (B,) and (lens.is_contiguous() or B <= 1)
+    assert lens.dtype == torch.int32 and lens.dim() == 1 and lens.shape[0] == B and (B <= 1 or lens.stride(0) == 1), "seq_lens: int32 [B]"
+
+
+def _q_ok(q, out, pool, Hkv, D):
+    """(rows, G, dtype code, row strides of q and out)"""
+    n, Hq, Dq = q.shape
+    assert q.dtype == pool.dtype == out.dtype and Dq == D and Hq > 0 and Hq % Hkv == 0, "q: [rows, G Hkv, D] of the pool's type"
+    qs, os_ = q.stride(), out.stride()
+    assert qs[2] == 1 and (qs[1] == D or Hq == 1) and out.shape[0] == n and out.numel() == n * Hq * D and os_[-1] == 1 and \
+        (len(os_) == 2 or os_[1] == D or Hq == 1), "out: [rows, G Hkv D]"
+    return n, Hq // Hkv, DTYPES[q.dtype], qs[0] if n > 1 else 0, os_[0] if n > 1 else 0
 
 
 def write(kv, slots, pool):
-    """kv [T, 2 Hkv, D] (K rows of all heads, then V rows; any token and row strides that are multiples of 8 elements) ->
-    pool at slots int64 [T] (slot = page_id * page + offset; < 0 or past the pool skipped).  The slots must be distinct."""
-    T = kv.shape[0]
-    _pool_ok(pool)
-    npg, Hkv, _, page, D = pool.shape
-    assert kv.dtype == pool.dtype and tuple(kv.shape) == (T, 2 * Hkv, D) and kv.stride(2) == 1, "kv: [T, 2 Hkv, D] of the pool's type"
-    assert slots.dtype == torch.int64 and slots.shape == (T,) and (slots.is_contiguous() or T <= 1)
+    """kv [T, 2 Hkv, D] (K rows of all heads, then V rows; 16-byte aligned rows, any token and row strides that are multiples of
+    8 elements) -> pool at slots int64 [T] (slot = page_id * page + offset; < 0 or past the pool skipped).  The slots that are
+    written must be distinct."""
+    npg, Hkv, page, D = _pool_ok(pool)
+    T, rows, Dk = kv.shape
+    st = kv.stride()
+    assert kv.dtype == pool.dtype and rows == 2 * Hkv and Dk == D and st[2] == 1, "kv: [T, 2 Hkv, D] of the pool's type"
+    assert slots.dtype == torch.int64 and slots.dim() == 1 and slots.shape[0] == T and (T <= 1 or slots.stride(0) == 1), "slots: int64 [T]"
     if T == 0:
         return
-    _here(kv, slots, pool)
-    assert kv.stride(0) % 8 == 0 and kv.stride(1) % 8 == 0 and kv.data_ptr() % 16 == 0, "kv rows must be 16-byte aligned"
-    _check(lib().k16_write(kv.data_ptr(), kv.stride(0), kv.stride(1), slots.data_ptr(), T, Hkv, D, page, npg, pool.data_ptr(),
-                           _stream()), "k16_write")
-
-
-def _q_ok(q, out, pool):
-    n, Hq, D = q.shape
-    Hkv = pool.shape[1]
-    assert q.dtype == pool.dtype == out.dtype and D == pool.shape[4] and Hq % Hkv == 0 and Hq > 0, "q: [rows, G Hkv, D] of the pool's type"
-    assert q.stride(2) == 1 and (q.stride(1) == D or Hq == 1) and q.data_ptr() % 16 == 0 and (q.stride(0) % 8 == 0 or n <= 1)
-    assert out.shape[0] == n and out.numel() == n * Hq * D and out.stride(-1) == 1 and (out.dim() == 2 or out.stride(1) == D or Hq == 1)
-    assert out.data_ptr() % 16 == 0 and (out.stride(0) % 8 == 0 or n <= 1), "q and out rows must be 16-byte aligned"
-    return Hq // Hkv
+    stream = _stream(kv, slots, pool)
+    _check(lib().k16_write(kv.data_ptr(), st[0] if T > 1 else 0, st[1], slots.data_ptr(), T, Hkv, D, page, npg, pool.data_ptr(), stream),
+           "k16_write")
 
 
 def attn(q, pool, block_table, seq_lens, out, ws, qscale, window=0, sinks=0, weights=None):
-    """q [B, G Hkv, D] -> out [B, G Hkv D] (or [B, G Hkv, D]); block_table int32 [B, width] (row stride 0 allowed), seq_lens
-    int32 [B]; qscale = softmax scale * log2(e).  Key j is seen when j < len and (window <= 0 or j >= len - window or
-    j < sinks); a row that sees no key gives zeros.  weights fp32 [B, Hkv, >= width * page] or None: the softmax weights of
-    every seen key, summed over the G heads, are added to it."""
-    B, Hq, D = q.shape
-    _pool_ok(pool)
-    G = _q_ok(q, out, pool)
-    npg, Hkv, _, page, _ = pool.shape
-    _table_ok(block_table, B)
+    """q [B, G Hkv, D] -> out [B, G Hkv D] (or [B, G Hkv, D]), rows 16-byte aligned; block_table int32 [B, width] (row stride 0
+    allowed), seq_lens int32 [B]; qscale = softmax scale * log2(e).  Key j is seen when j < len and (window <= 0 or
+    j >= len - window or j < sinks); a row that sees no key gives zeros.  weights fp32 [B, Hkv, >= width * page] or None: the
+    softmax weights of every seen key, summed over the G heads, are added to it."""
+    npg, Hkv, page, D = _pool_ok(pool)
+    B, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)
+    width, bs = _table_ok(block_table, B)
     _lens_ok(seq_lens, B)
     if B == 0:
         return
-    width = block_table.shape[1]
+    stream = _stream(q, pool, block_table, seq_lens, out, ws.buf)
     wp = wb = wh = 0
     if weights is not None:
-        assert weights.dtype == torch.float32 and weights.shape[:2] == (B, Hkv) and weights.shape[2] >= width * page
-        assert weights.stride(2) == 1, "weights: fp32 [B, Hkv, >= width * page]"
-        _here(weights)
-        wp, wb, wh = weights.data_ptr(), weights.stride(0), weights.stride(1)
-    _here(q, pool, block_table, seq_lens, out, ws.buf)
-    _check(lib().k16_attn(DTYPES[q.dtype], q.data_ptr(), q.stride(0) if B > 1 else 0, pool.data_ptr(), npg, block_table.data_ptr(),
-                          block_table.stride(0), width, seq_lens.data_ptr(), B, Hkv, G, D, page, qscale, window, sinks, wp, wb, wh,
-                          ws.tickets.data_ptr(), ws.ntickets, ws.buf.data_ptr(), ws.nbytes, out.data_ptr(),
-                          out.stride(0) if B > 1 else 0, _stream()), "k16_attn")
+        assert weights.dtype == torch.float32 and weights.dim() == 3, "weights: fp32 [B, Hkv, >= width * page]"
+        (wB, wH, W), (wb, wh, w1) = weights.shape, weights.stride()
+        assert wB == B and wH == Hkv and W >= width * page and (w1 == 1 or W <= 1), "weights: fp32 [B, Hkv, >= width * page]"
+        _stream(weights)
+        wp = weights.data_ptr()
+    _check(lib().k16_attn(dt, q.data_ptr(), qs, pool.data_ptr(), npg, block_table.data_ptr(), bs, width, seq_lens.data_ptr(), B, Hkv, G,
+                          D, page, qscale, window, sinks, wp, wb, wh, ws.ptickets, ws.ntickets, ws.pbuf, ws.nbytes, out.data_ptr(),
+                          os_, stream), "k16_attn")
 
 
 def prefill(q, cu_q, pool, block_table, seq_lens, out, qscale, window=0, sinks=0, ws=None):
-    """q [T, G Hkv, D] -> out [T, G Hkv D]: row b's new tokens are rows cu_q[b] .. cu_q[b + 1] (int32 [B + 1]) and the last ones
-    of its seq_lens[b] cached tokens (their keys and values are in the pages already).  The token at position p sees key
-    j <= p when window <= 0 or j > p - window or j < sinks; one at a negative position gives zeros; rows of out that belong
-    to no sequence are left as they are.  The cached rows within seq_lens must be finite."""
-    T = q.shape[0]
+    """q [T, G Hkv, D] -> out [T, G Hkv D], rows 16-byte aligned: row b's new tokens are rows cu_q[b] .. cu_q[b + 1] (int32
+    [B + 1]) and the last ones of its seq_lens[b] cached tokens (their keys and values are in the pages already).  The token
+    at position p sees key j <= p when window <= 0 or j > p - window or j < sinks; one at a negative position gives zeros;
+    rows of out that belong to no sequence are left as they are.  The cached rows within seq_lens must be finite.  ws: a
+    Workspace made with new_tokens."""
+    npg, Hkv, page, D = _pool_ok(pool)
+    T, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)
     B = block_table.shape[0]
-    _pool_ok(pool)
-    G = _q_ok(q, out, pool)
-    npg, Hkv, _, page, D = pool.shape
-    _table_ok(block_table, B)
+    width, bs = _table_ok(block_table, B)
     _lens_ok(seq_lens, B)
-    assert cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous()
+    assert cu_q.dtype == torch.int32 and cu_q.dim() == 1 and cu_q.shape[0] == B + 1 and cu_q.stride(0) == 1, "cu_q: int32 [B + 1]"
     if B == 0 or T == 0:
         return
-    _here(q, cu_q, pool, block_table, seq_lens, out, ws.buf)
-    _check(lib().k16_prefill(DTYPES[q.dtype], q.data_ptr(), q.stride(0) if T > 1 else 0, T, cu_q.data_ptr(), pool.data_ptr(), npg,
-                             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B, Hkv, G, D,
-                             page, qscale, window, sinks, ws.tickets.data_ptr(), ws.ntickets, ws.buf.data_ptr(), ws.nbytes,
-                             out.data_ptr(), out.stride(0) if T > 1 else 0, _stream()), "k16_prefill")
+    assert ws is not None, "ws: a Workspace made with new_tokens"
+    stream = _stream(q, cu_q, pool, block_table, seq_lens, out, ws.buf)
+    _check(lib().k16_prefill(dt, q.data_ptr(), qs, T, cu_q.data_ptr(), pool.data_ptr(), npg, block_table.data_ptr(), bs, width,
+                             seq_lens.data_ptr(), B, Hkv, G, D, page, qscale, window, sinks, ws.ptickets, ws.ntickets, ws.pbuf,
+                             ws.nbytes, out.data_ptr(), os_, stream), "k16_prefill")
 
 
 def evict(pool, block_table, seq_lens, weights, budget, sinks, recent, kept, new_lens, new_weights, dst_pool=None,
@@ -203,33 +203,35 @@ def evict(pool, block_table, seq_lens, weights, budget, sinks, recent, kept, new
     min(len, budget); new_weights fp32 [B, Hkv, >= budget]: their weights, then zeros (it must not overlap weights).
     Without dst_table the rows move to the front of the row's own pages (pages must not be shared between rows); with
     it they are copied to the pages of dst_table in dst_pool (default: pool), which must not be among the pages read."""
-    _pool_ok(pool)
-    npg, Hkv, _, page, D = pool.shape
+    npg, Hkv, page, D = _pool_ok(pool)
     B = block_table.shape[0]
-    _table_ok(block_table, B)
+    width, bs = _table_ok(block_table, B)
     _lens_ok(seq_lens, B)
-    assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, Hkv) and weights.stride(2) == 1
+    assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, Hkv), "weights: fp32 [B, Hkv, W]"
+    (wb, wh, w1), W = weights.stride(), weights.shape[2]
+    assert w1 == 1 or W <= 1
     assert budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, "sinks + recent must fit the budget"
-    assert kept.dtype == torch.int32 and kept.shape == (B, Hkv, budget) and kept.is_contiguous()
-    assert new_lens.dtype == torch.int32 and new_lens.shape == (B,) and new_lens.is_contiguous()
+    assert kept.dtype == torch.int32 and kept.shape == (B, Hkv, budget) and kept.is_contiguous(), "kept: int32 [B, Hkv, budget]"
+    assert new_lens.dtype == torch.int32 and new_lens.shape == (B,) and new_lens.is_contiguous(), "new_lens: int32 [B]"
     assert new_weights.dtype == torch.float32 and new_weights.is_contiguous() and new_weights.dim() == 3
-    assert new_weights.shape[:2] == (B, Hkv) and new_weights.shape[2] >= budget
-    assert new_weights.data_ptr() != weights.data_ptr(), "new_weights must not overlap weights"
+    assert new_weights.shape[:2] == (B, Hkv) and new_weights.shape[2] >= budget, "new_weights: fp32 [B, Hkv, >= budget]"
     if B == 0:
         return
+    nwp, wp = new_weights.data_ptr(), weights.data_ptr()
+    assert nwp + new_weights.numel() * 4 <= wp or wp + ((B - 1) * wb + (Hkv - 1) * wh + W) * 4 <= nwp, "new_weights overlaps weights"
+    assert new_lens.data_ptr() != seq_lens.data_ptr(), "new_lens must not be seq_lens"
+    stream = _stream(pool, block_table, seq_lens, weights, kept, new_lens, new_weights)
     dp = dn = dt = ds = dw = 0
     if dst_table is not None:
         dst = pool if dst_pool is None else dst_pool
-        _pool_ok(dst)
-        assert dst.dtype == pool.dtype and dst.shape[1:] == pool.shape[1:], "dst_pool: another pool of the same kind"
-        _table_ok(dst_table, B)
-        assert dst_table.shape[1] * page >= budget, "dst_table must cover the budget"
-        _here(dst, dst_table)
-        dp, dn, dt, ds, dw = dst.data_ptr(), dst.shape[0], dst_table.data_ptr(), dst_table.stride(0), dst_table.shape[1]
+        dn, dH, dpage, dD = _pool_ok(dst)
+        assert dst.dtype == pool.dtype and (dH, dpage, dD) == (Hkv, page, D), "dst_pool: another pool of the same kind"
+        dw, ds = _table_ok(dst_table, B)
+        assert dw * page >= budget, "dst_table must cover the budget"
+        _stream(dst, dst_table)
+        dp, dt = dst.data_ptr(), dst_table.data_ptr()
     else:
         assert dst_pool is None, "dst_pool needs a dst_table"
-    _here(pool, block_table, seq_lens, weights, kept, new_lens, new_weights)
-    _check(lib().k16_evict(pool.data_ptr(), npg, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                           seq_lens.data_ptr(), B, Hkv, D, page, weights.data_ptr(), weights.stride(0), weights.stride(1),
-                           weights.shape[2], budget, sinks, recent, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
-                           new_weights.shape[2], dp, dn, dt, ds, dw, _stream()), "k16_evict")
+    _check(lib().k16_evict(pool.data_ptr(), npg, block_table.data_ptr(), bs, width, seq_lens.data_ptr(), B, Hkv, D, page, wp, wb, wh, W,
+                           budget, sinks, recent, kept.data_ptr(), new_lens.data_ptr(), nwp, new_weights.shape[2], dp, dn, dt, ds, dw,
+                           stream), "k16_evict")
