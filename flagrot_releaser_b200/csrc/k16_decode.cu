@@ -18,6 +18,7 @@
 // other 8 carry, in the second product, the rounding errors of the weights: p = hi + lo, both of the cache's type, at no
 // extra cost, so a weight meets the values with an error of 2^-17 instead of 2^-9.
 #include "k16_kernels.h"
+#include "k16_launch.cuh"
 #include "k16_tma.cuh"
 
 namespace k16 {
@@ -30,6 +31,9 @@ constexpr int MAX_GT = 32;               // q heads per segment
 constexpr float LAZY = 8.f;              // the softmax reference moves when a score exceeds it by more than this (log2)
 
 __device__ int g_status;
+
+// a workspace slot: sums [GT][D], then (reference, denominator) [GT]; a multiple of 16 bytes
+__host__ __device__ __forceinline__ long long slot_floats(int GT, int D) { return (static_cast<long long>(GT) * (D + 2) + 3) & ~3ll; }
 
 template <int D> struct Smem {
   // a multiple of NW: a stage always goes to the same warps, whose waits on its barrier then follow its phases one by one
@@ -145,6 +149,80 @@ FR_DEVI void wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort, in
 }
 #define k16_wait(bar, parity, abort) wait_at(bar, parity, abort, __LINE__)
 
+// The pieces of CTAs c0 .. c1 of the segment that begins at f0, in order: four dims of a head per thread, eight pieces in flight;
+// few heads: the threads also share the pieces, and their sums meet in shared memory (scr).
+template <int DT, int D>
+FR_DEVI void join(const AttnArgs& a, const float* part, long long quota, long long f0, int c0, int c1, int heads, int GT, float* scr,
+                  uint16_t* out, float* lse) {
+  constexpr int NTH = 32 * NW, IN = 8;
+  const int cols = heads * (D / 4), tid = threadIdx.x, sets = max(NTH / cols, 1), stride = sets > 1 ? cols * sets : NTH;
+  const auto finish = [&](int col, float M, float L, float4 v) {
+    const float inv = 1.f / L;
+    uint2 r;
+    r.x = Elem<DT>::pack(v.x * inv, v.y * inv);
+    r.y = Elem<DT>::pack(v.z * inv, v.w * inv);
+    *reinterpret_cast<uint2*>(out + 4 * col) = r;              // (col = head * D / 4 + dims)
+    if (lse && col % (D / 4) == 0) lse[col / (D / 4)] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
+  };
+  for (int i = tid; i < (sets > 1 ? stride : cols); i += stride) {
+    const int col = i % cols, set = i / cols, hh = col / (D / 4), d = 4 * (col - hh * (D / 4));
+    float M = -INFINITY, L = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0 + set; c <= c1; c += IN * sets) {
+      float2 e[IN];
+      float4 y[IN];
+#pragma unroll
+      for (int k = 0; k < IN; ++k) {
+        const int cc = c + k * sets;
+        const float* p = part + (static_cast<long long>(cc) * 2 + (cc == c0 && f0 != c0 * quota ? 1 : 0)) * slot_floats(GT, D);
+        e[k] = cc <= c1 ? __ldcg(reinterpret_cast<const float2*>(p + GT * D + 2 * hh)) : make_float2(-INFINITY, 0.f);
+        y[k] = cc <= c1 ? __ldcg(reinterpret_cast<const float4*>(p + hh * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float nm = M;
+#pragma unroll
+      for (int k = 0; k < IN; ++k) nm = fmaxf(nm, e[k].x);
+      const float f = ex2(M - nm);
+      M = nm;
+      L *= f;
+      v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+#pragma unroll
+      for (int k = 0; k < IN; ++k) {
+        const float x = ex2(e[k].x - nm);
+        L = fmaf(x, e[k].y, L);
+        v.x = fmaf(x, y[k].x, v.x);
+        v.y = fmaf(x, y[k].y, v.y);
+        v.z = fmaf(x, y[k].z, v.z);
+        v.w = fmaf(x, y[k].w, v.w);
+      }
+    }
+    if (sets == 1) {
+      finish(col, M, L, v);
+    } else {
+      *reinterpret_cast<float4*>(scr + 4 * i) = v;
+      *reinterpret_cast<float2*>(scr + 4 * NTH + 2 * i) = make_float2(M, L);
+    }
+  }
+  if (sets == 1) return;                                       // (all threads)
+  bar_consumers();
+  if (tid < cols) {
+    float M = -INFINITY, L = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int n = min(sets, c1 - c0 + 1);                      // the others had no piece
+    for (int s = 0; s < n; ++s) M = fmaxf(M, scr[4 * NTH + 2 * (s * cols + tid)]);
+    for (int s = 0; s < n; ++s) {
+      const float2 e = *reinterpret_cast<const float2*>(scr + 4 * NTH + 2 * (s * cols + tid));
+      const float4 y = *reinterpret_cast<const float4*>(scr + 4 * (s * cols + tid));
+      const float x = ex2(e.x - M);
+      L = fmaf(x, e.y, L);
+      v.x = fmaf(x, y.x, v.x);
+      v.y = fmaf(x, y.y, v.y);
+      v.z = fmaf(x, y.z, v.z);
+      v.w = fmaf(x, y.w, v.w);
+    }
+    finish(tid, M, L, v);
+  }
+}
+
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map, int nhg,
                                                        float* part, float* lse, float* scores, long long score_ld) {
@@ -171,7 +249,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
     *abort = 0;
     tma_prefetch_map(&map);
   }
-  if (scores) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  let_next_start();
+  after_previous();
   // the list's length; rows that see nothing are written as zeros here
   long long total = 0;
   for (int b = tid; b < a.B; b += THREADS) {
@@ -357,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
       for (int x = 0; x < ND; ++x) *reinterpret_cast<float2*>(mw + x * 8) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
     bar_consumers();
     const int c0 = wk.first_cta(), c1 = wk.last_cta();
-    float* slot = part + (static_cast<long long>(blockIdx.x) * 2 + (wk.f0 + wk.k0 == blockIdx.x * quota ? 0 : 1)) * (GT * (D + 2));
+    float* slot = part + (static_cast<long long>(blockIdx.x) * 2 + (wk.f0 + wk.k0 == blockIdx.x * quota ? 0 : 1)) * slot_floats(GT, D);
     for (int i = tid; i < heads * (D / 2); i += 32 * NW) {
       const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2)), w0 = (hh >> 3) * GROUPS;
       float M = -INFINITY, L = 0.f;
@@ -394,38 +473,21 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
         __threadfence();
       }
       bar_consumers();
-      if (*flag) {
-        for (int i = tid; i < heads * (D / 2); i += 32 * NW) {
-          const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2));
-          float M = -INFINITY, L = 0.f;
-          float2 v = make_float2(0.f, 0.f);
-          for (int c = c0; c <= c1; ++c) {
-            const float* p = part + (static_cast<long long>(c) * 2 + (c == c0 && wk.f0 != c0 * quota ? 1 : 0)) * (GT * (D + 2));
-            const float2 e = __ldcg(reinterpret_cast<const float2*>(p + GT * D + 2 * hh));
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + hh * D + d));
-            const float nm = fmaxf(M, e.x), f = ex2(M - nm), x = ex2(e.x - nm);
-            M = nm;
-            L = L * f + x * e.y;
-            v.x = v.x * f + x * y.x;
-            v.y = v.y * f + x * y.y;
-          }
-          const float inv = 1.f / L;
-          reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + wk.b * a.o_bs + (hq0 + hh) * D)[d >> 1] = Elem<DT>::pack(v.x * inv, v.y * inv);
-          if (lse && d == 0) lse[static_cast<long long>(wk.b) * Hq + hq0 + hh] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
-        }
-      }
+      if (*flag) join<DT, D>(a, part, quota, wk.f0, c0, c1, heads, GT, mo, static_cast<uint16_t*>(a.out) + wk.b * a.o_bs + hq0 * D,
+                             lse ? lse + static_cast<long long>(wk.b) * Hq + hq0 : nullptr);
     }
     bar_consumers();                                           // the merge area and the flag are free again
   }
 }
 
 // weights[b, h, j] += sum over the head group of 2^(score - lse): four keys per thread; VEC: the weights' rows are 16-byte
-// aligned.  Launched behind k_decode's start (programmatic launch).
+// aligned.
 template <bool VEC> __global__ void __launch_bounds__(256) k_weights(AttnArgs a, const float* scores, long long score_ld, const float* lse, int chunks) {
   const int bh = blockIdx.x / chunks, b = bh / a.c.Hkv, h = bh - b * a.c.Hkv, Hq = a.c.Hkv * a.G;
+  let_next_start();
+  after_previous();
   const int len = a.c.len(b), j = (blockIdx.x - bh * chunks) * 1024 + 4 * threadIdx.x;
   const Span sp(len - 1, a.window, a.sinks);
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   if (j >= len || (j >= sp.s1 && j + 4 <= sp.lo)) return;
   float* w = a.weights + b * a.w_bs + h * a.w_hs + j;
   const bool all = j + 4 <= len && (j >= sp.lo || j + 4 <= sp.s1);
@@ -455,26 +517,25 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_weights(AttnArgs a,
 long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
 template <int DT, int D, int NT>
-cudaError_t launch(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
+cudaError_t launch_d(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                    cudaStream_t st) {
   const auto k = k_decode<DT, D, NT>;
   static std::atomic<bool> done[MAX_DEVICES];
   if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, map, nhg, part, lse, scores, ld);
-  return cudaGetLastError();
+  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, map, nhg, part, lse, scores, ld);
 }
 template <int DT, int D>
 cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                       cudaStream_t st) {
-  if (a.G <= 8) return launch<DT, D, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
-  if (a.G <= 16) return launch<DT, D, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
-  return launch<DT, D, 4>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 8) return launch_d<DT, D, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 16) return launch_d<DT, D, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  return launch_d<DT, D, 4>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
 }
 
 }  // namespace
 
 // partials of two pieces per CTA | lse [rows, Hq] | scores [rows, Hq, max_len rounded up to blocks]
-static long long part_bytes(int G, int D) { return up(2ll * MAX_CTAS * (G < MAX_GT ? G : MAX_GT) * (D + 2) * 4, 256); }
+static long long part_bytes(int G, int D) { return up(2ll * MAX_CTAS * slot_floats(G < MAX_GT ? G : MAX_GT, D) * 4, 256); }
 long long attn_ws_bytes(int rows, int Hkv, int G, int D, long long max_len, int weights) {
   const long long r = static_cast<long long>(rows) * Hkv * G;
   return part_bytes(G, D) + (weights ? up(r * 4, 256) + r * up(max_len, BLK) * 4 : 0);
@@ -506,17 +567,8 @@ cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st) {
   const long long chunks = (width + 1023) / 1024;
   if (chunks * a.B * a.c.Hkv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   const bool vec = (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0 && a.w_bs % 4 == 0 && a.w_hs % 4 == 0;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(static_cast<unsigned>(chunks * a.B * a.c.Hkv));
-  c.blockDim = dim3(256);
-  c.stream = st;
-  c.attrs = &at;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, vec ? k_weights<true> : k_weights<false>, a, static_cast<const float*>(scores), ld,
-                            static_cast<const float*>(lse), static_cast<int>(chunks));
+  return launch(vec ? k_weights<true> : k_weights<false>, static_cast<unsigned>(chunks * a.B * a.c.Hkv), 256, 0, 0, true, st, a,
+                static_cast<const float*>(scores), ld, static_cast<const float*>(lse), static_cast<int>(chunks));
 }
 
 }  // namespace k16

@@ -1,7 +1,7 @@
 // Eviction from the 16-bit cache: per (row, kv head) the tokens with the largest accumulated attention weight stay, in order.
 //
 // HBM bound: 8 D bytes move per kept (token, kv head) (key and value row, read and written), 4 bytes are read per weight.
-// Two launches, the second one's start hidden behind the first (programmatic launch):
+// Two launches:
 //   k_select  a cluster of 1 to 8 CTAs per (row, kv head): the threshold by a radix search over order-preserving keys (11, 11
 //             and 10 bits; the CTAs' histograms are added through distributed shared memory), then one scan that writes the
 //             kept positions and their weights;
@@ -11,7 +11,7 @@
 #include <cooperative_groups.h>
 
 #include "k16_kernels.h"
-#include "k16_tma.cuh"
+#include "k16_launch.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -63,7 +63,7 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   };
   const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int b = g / a.c.Hkv, h = g - b * a.c.Hkv;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  let_next_start();
   const int len = min(a.c.len(b), a.w_len), m = min(len, a.budget);
   const float* w = a.weights + b * a.w_bs + h * a.w_hs;
   int* kept = a.kept + static_cast<long long>(g) * a.budget;
@@ -218,15 +218,14 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   if (CL) sync();                                     // the others have read this CTA's counts
 }
 
-FR_DEVI void wait_select() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
-
 // Rows to other pages: a CTA copies TOK kept tokens, 16-byte pieces, eight of each thread's in flight.
 constexpr int CT = 256, TOK = 64;
 template <int D> __global__ void __launch_bounds__(CT) k_copy(EvictArgs a, int chunks) {
   constexpr int PPR = D / 8, PPT = 2 * PPR;           // pieces per row, per token (key row, then value row)
   __shared__ long long src[TOK], dst[TOK];            // element offsets of the key rows, or -1 | -2
   const int g = blockIdx.x / chunks, b = g / a.c.Hkv, h = g - b * a.c.Hkv, r0 = (blockIdx.x - g * chunks) * TOK;
-  wait_select();
+  let_next_start();
+  after_previous();
   const int m = a.new_lens[b];
   if (r0 >= m) return;
   const int n = min(TOK, m - r0);
@@ -265,7 +264,8 @@ template <int D> __global__ void __launch_bounds__(NT) k_move(EvictArgs a, int C
   constexpr int PPR = D / 8, PPT = 2 * PPR, IT = 8, R = IT * NT / PPT;   // tokens per CTA and step
   cg::cluster_group cl = cg::this_cluster();
   const int g = blockIdx.x / C, rank = blockIdx.x - g * C, b = g / a.c.Hkv, h = g - b * a.c.Hkv;
-  wait_select();
+  let_next_start();
+  after_previous();
   const int len = min(a.c.len(b), a.w_len), m = a.new_lens[b];
   if (len <= a.budget) return;                        // (the whole cluster)
   const int* kept = a.kept + static_cast<long long>(g) * a.budget;
@@ -314,30 +314,6 @@ template <int D> __global__ void __launch_bounds__(NT) k_move(EvictArgs a, int C
 #pragma unroll
       for (int i = 0; i < IT; ++i) x[i] = y[i], moved[i] = my[i];
   }
-}
-
-template <class... Ts>
-cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, size_t smem, int cluster, bool dependent, cudaStream_t st,
-                   Ts... args) {
-  cudaLaunchAttribute at[2];
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(grid);
-  c.blockDim = dim3(threads);
-  c.stream = st;
-  c.dynamicSmemBytes = smem;
-  c.attrs = at;
-  if (cluster > 0) {
-    at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[c.numAttrs].val.clusterDim.x = cluster;
-    at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
-    ++c.numAttrs;
-  }
-  if (dependent) {
-    at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++c.numAttrs;
-  }
-  return cudaLaunchKernelEx(&c, k, args...);
 }
 
 // CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each, and to hold the keys in shared memory

@@ -17,6 +17,7 @@
 // P is rounded to the cache's type (2^-9 relative in bf16, 2^-12 in fp16: one rounding, like the output's own); the row sums,
 // S and O are 32-bit.
 #include "k16_kernels.h"
+#include "k16_launch.cuh"
 #include "k16_tma.cuh"
 
 namespace k16 {
@@ -185,6 +186,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     tma_prefetch_map(&qmap);
     tma_prefetch_map(&kvmap);
   }
+  let_next_start();
+  after_previous();
   if (w == W_MMA) {
     tc5::tmem_alloc(sm + S::MISC, 512);
     tc5::tmem_relinquish();
@@ -640,12 +643,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 }
 
 template <int DT, int D>
-cudaError_t launch(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int dev, int grid, cudaStream_t st) {
+cudaError_t launch_p(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int dev, int grid, cudaStream_t st) {
   const auto k = k_prefill<DT, D>;
   static std::atomic<bool> done[MAX_DEVICES];
   if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  k<<<grid, THREADS, Smem<D>::TOTAL, st>>>(a, qm, kv, hb, nhg, box);
-  return cudaGetLastError();
+  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, qm, kv, hb, nhg, box);
 }
 
 }  // namespace
@@ -686,8 +688,8 @@ cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
   const long long items = max_pairs(a.B, a.c.Hkv, a.G, a.T) * MAX_SPLIT;
   const int grid = static_cast<int>(items < sms ? items : sms);
   if (dtype == 0)
-    return a.D == 128 ? launch<0, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch<0, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
-  return a.D == 128 ? launch<1, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch<1, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
+    return a.D == 128 ? launch_p<0, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch_p<0, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
+  return a.D == 128 ? launch_p<1, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch_p<1, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
 }
 
 }  // namespace k16

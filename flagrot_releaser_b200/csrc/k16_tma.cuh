@@ -8,8 +8,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
-
 #include "fr_tc5.cuh"
 
 namespace k16 {
@@ -28,25 +26,6 @@ inline EncodeFn encode_fn() {
     return reinterpret_cast<EncodeFn>(p);
   }();
   return fn;
-}
-
-// What a launch needs to know about the current device, looked up once per device: its SMs, and that a kernel may use its
-// dynamic shared memory (the attribute belongs to the kernel on one device).
-constexpr int MAX_DEVICES = 64;
-inline cudaError_t device_sms(int& dev, int& sms) {
-  static std::atomic<int> known[MAX_DEVICES];
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
-  sms = dev < MAX_DEVICES ? known[dev].load(std::memory_order_relaxed) : 0;
-  if (sms > 0) return cudaSuccess;
-  const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess && dev < MAX_DEVICES) known[dev].store(sms, std::memory_order_relaxed);
-  return e;
-}
-template <class K> cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<bool> (&done)[MAX_DEVICES]) {
-  if (dev < MAX_DEVICES && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < MAX_DEVICES) done[dev].store(true, std::memory_order_relaxed);
-  return e;
 }
 
 // box of 64 elements x `mid` x `outer`; dims and byte strides of the two outer axes

@@ -1,6 +1,7 @@
 // Row writer of the 16-bit cache: a copy of 16-byte pieces from the projection's output to the pages.  HBM bound (every byte is
 // read once and written once); a decode step's few rows are bound by the launch.
 #include "k16_kernels.h"
+#include "k16_launch.cuh"
 
 namespace k16 {
 namespace {
@@ -8,15 +9,17 @@ namespace {
 // A CTA copies PER * CT consecutive pieces (piece = token, row, 16 bytes of it), PER of them in flight per thread.
 constexpr int CT = 256;
 template <int PER>
-__global__ void __launch_bounds__(CT) k_write(const uint16_t* __restrict__ kv, long long kv_ts, long long kv_hs,
-                                              const long long* __restrict__ slots, int T, int Hkv, int D, int page_sh, long long nslots,
-                                              uint16_t* __restrict__ pool) {
+__global__ void __launch_bounds__(CT) k_write(const uint16_t* kv, long long kv_ts, long long kv_hs,
+                                              const long long* slots, int T, int Hkv, int D, int page_sh, long long nslots,
+                                              uint16_t* pool) {
   const int psh = D == 128 ? 4 : 3, ppt = 2 * Hkv << psh;      // pieces per row (log2), per token
   const long long first = static_cast<long long>(blockIdx.x) * (PER * CT);
   const int tok0 = static_cast<int>(first / ppt);
   const unsigned rem = static_cast<unsigned>(first - static_cast<long long>(tok0) * ppt) + threadIdx.x;
   uint4 x[PER];
   uint16_t* to[PER];
+  let_next_start();
+  after_previous();
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const unsigned p = rem + i * CT, dt = p / ppt, r = p - dt * ppt;
@@ -39,11 +42,9 @@ __global__ void __launch_bounds__(CT) k_write(const uint16_t* __restrict__ kv, l
 cudaError_t write_rows(const uint16_t* kv, long long kv_ts, long long kv_hs, const long long* slots, int T, int Hkv, int D,
                        int page_sh, long long num_pages, uint16_t* pool, cudaStream_t st) {
   const long long n = static_cast<long long>(T) * 2 * Hkv * (D >> 3), nslots = num_pages << page_sh;
-  if (n > 148ll * 8 * 4 * CT)          // more than one piece for every thread the SMs hold: four in flight per thread
-    k_write<4><<<static_cast<unsigned>((n + 4 * CT - 1) / (4 * CT)), CT, 0, st>>>(kv, kv_ts, kv_hs, slots, T, Hkv, D, page_sh, nslots, pool);
-  else
-    k_write<1><<<static_cast<unsigned>((n + CT - 1) / CT), CT, 0, st>>>(kv, kv_ts, kv_hs, slots, T, Hkv, D, page_sh, nslots, pool);
-  return cudaGetLastError();
+  const int per = n > 148ll * 8 * 4 * CT ? 4 : 1;   // more than one piece for every thread the SMs hold: four in flight
+  return launch(per == 4 ? k_write<4> : k_write<1>, static_cast<unsigned>((n + per * CT - 1) / (per * CT)), CT, 0, 0, true, st, kv, kv_ts, kv_hs,
+                slots, T, Hkv, D, page_sh, nslots, pool);
 }
 
 }  // namespace k16
