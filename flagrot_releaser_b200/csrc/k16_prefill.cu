@@ -66,8 +66,8 @@ template <int D> struct Smem {
   static constexpr int STAGE = BN * D * 2;                     // one K or V tile
   static constexpr int STAGES = D == 128 ? 5 : 10;
   static constexpr int RING = 2 * QT;
-  static constexpr int BAR = RING + STAGES * STAGE;            // full[STAGES] empty[STAGES] qfull qempty sfull[2] pfull[2][2] ofull[2]
-  static constexpr int NBAR = 2 * STAGES + 2 + 8 + 4 + 2;          // ... items: full[2], empty[2]; tile sync[2]
+  static constexpr int BAR = RING + STAGES * STAGE;            // full[STAGES] empty[STAGES] qfull qempty sfull[2][2] pfull[2][2] ofull[2]
+  static constexpr int NBAR = 2 * STAGES + 2 + 10 + 4 + 2 + 2;          // ... items: full[2], empty[2]; tile sync[2], pvdone[2]
   static constexpr int ITEMS = BAR + NBAR * 8;                 // Item[2]
   static constexpr int MISC = ITEMS + 2 * 64;                  // tensor-memory base, abort flag
   static constexpr int TOTAL = MISC + 16 + 1024;
@@ -132,22 +132,48 @@ FR_DEVI float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// the registers of an earlier tmem_ld32 hold their values from here on
+FR_DEVI void ld_wait(uint32_t (&v)[32]) {
+#define K16_RW4(o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3])
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : K16_RW4(0), K16_RW4(4), K16_RW4(8), K16_RW4(12), K16_RW4(16), K16_RW4(20), K16_RW4(24), K16_RW4(28)::"memory");
+#undef K16_RW4
+}
+// scores of hidden keys -> -inf
+FR_DEVI void hide(uint32_t (&v)[32], uint32_t see) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!(see & (1u << e))) v[e] = 0xFF800000u;
+}
 // the n lowest of 32 bits
 FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 FR_DEVI float4 f4(const uint32_t* v) {
   return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
 }
-template <int DT> FR_DEVI void put8(uint16_t* out, float4 x, float4 y, float inv, bool any) {
-  uint4 v = make_uint4(0, 0, 0, 0);
+// 16 dims of an output row times inv (zeros when !any); wide: rows are 32-byte aligned, a whole sector per store
+template <int DT> FR_DEVI void put16(uint16_t* out, float4 x, float4 y, float4 z, float4 t, float inv, bool any, bool wide) {
+  uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (any) {
-    v.x = Elem<DT>::pack(x.x * inv, x.y * inv);
-    v.y = Elem<DT>::pack(x.z * inv, x.w * inv);
-    v.z = Elem<DT>::pack(y.x * inv, y.y * inv);
-    v.w = Elem<DT>::pack(y.z * inv, y.w * inv);
+    v[0] = Elem<DT>::pack(x.x * inv, x.y * inv);
+    v[1] = Elem<DT>::pack(x.z * inv, x.w * inv);
+    v[2] = Elem<DT>::pack(y.x * inv, y.y * inv);
+    v[3] = Elem<DT>::pack(y.z * inv, y.w * inv);
+    v[4] = Elem<DT>::pack(z.x * inv, z.y * inv);
+    v[5] = Elem<DT>::pack(z.z * inv, z.w * inv);
+    v[6] = Elem<DT>::pack(t.x * inv, t.y * inv);
+    v[7] = Elem<DT>::pack(t.z * inv, t.w * inv);
   }
-  *reinterpret_cast<uint4*>(out) = v;
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(out), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(out)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(out)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
+
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
                                                         const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
@@ -158,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
   const uint32_t sm = (raw + 1023) & ~1023u;
   unsigned char* base = smem_raw + (sm - raw);
   const uint32_t full = sm + S::BAR, empty = full + 8 * STAGES, qfull = empty + 8 * STAGES, qempty = qfull + 8, sfull = qempty + 8,
-                 pfull = sfull + 16, ofull = pfull + 32, ifull = ofull + 16, iempty = ifull + 16, tsync = iempty + 16;
+                 pfull = sfull + 32, ofull = pfull + 32, ifull = ofull + 16, iempty = ifull + 16, tsync = iempty + 16, pvdone = tsync + 16;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base + S::MISC);
   volatile uint32_t* abort = tmem_slot + 1;
   volatile uint32_t* flag = tmem_slot + 2;                     // [2]: this CTA joins the pieces of the tile
@@ -173,7 +199,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     tc5::mbar_init(qfull, 1);
     tc5::mbar_init(qempty, 2);
     for (int i = 0; i < 2; ++i) {
-      tc5::mbar_init(sfull + 8 * i, 1);
+      tc5::mbar_init(sfull + 16 * i, 1);
+      tc5::mbar_init(sfull + 16 * i + 8, 1);
+      tc5::mbar_init(pvdone + 8 * i, 1);
       tc5::mbar_init(pfull + 16 * i, 4);
       tc5::mbar_init(pfull + 16 * i + 8, 4);
       tc5::mbar_init(ofull + 8 * i, 1);
@@ -361,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     if (*abort && lane == 0 && qc) tc5::mbar_wait(qfull, (qc - 1) & 1);
   } else if (w == W_MMA || w == W_MMA + 1) {                   // ------------------------------------- MMAs, a warp per tile
     // the softmax takes |qscale|: a negative scale negates the A operand
-    const uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, BN) | (a.qscale < 0.f ? A_NEGATE : 0u);
+    const uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, 64) | (a.qscale < 0.f ? A_NEGATE : 0u);
     constexpr uint32_t ID_PV = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, D) | B_MN_MAJOR;
     const int i = w - W_MMA;
     const uint32_t tSi = tS + i * 128, tOi = tO + i * 128, qlo = desc_lo(sm + i * S::QT, DESC_LO_K), pf = pfull + 16 * i;
@@ -386,62 +414,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         const int kb = k < it.k1 ? it.block(k) * BN : 0;
         const bool now = k < it.k1 && t.needs(kb);
         // Every tile of the ring is waited for, needed or not: the parity of a later phase would not tell.
+        const uint32_t sv = sm + S::RING + st * S::STAGE, vlo = desc_lo(sv, DESC_LO_MN), vbar = empty + 8 * st;
         if (k > it.k0) {
-          const uint32_t sv = sm + S::RING + st * S::STAGE, vlo = desc_lo(sv, DESC_LO_MN), vbar = empty + 8 * st;
           if (!(run = k16_wait(full + 8 * st, ph))) break;
           if (++st == STAGES) st = 0, ph ^= 1;
-          if (was) {
-            if (kbv + BN > it.len) {                           // values behind the sequence: 0 * NaN would be NaN
-              for (int j = (it.len - kbv) * 8 + lane; j < BN * 8; j += 32)
+          if (was && kbv + BN > it.len) {                      // values behind the sequence: 0 * NaN would be NaN
+            for (int j = (it.len - kbv) * 8 + lane; j < BN * 8; j += 32)
 #pragma unroll
-                for (int x = 0; x < HALVES; ++x)
-                  asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + j * 16), "r"(0) : "memory");
-              tc5::fence_async_smem();
-              __syncwarp();
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {                      // P comes in two halves of 64 keys
-              if (!(run = k16_wait(pf + 8 * c, pc & 1))) break;
-              tc5::fence_after_sync();
-              if (tc5::elect_one()) {
-#pragma unroll
-                for (int s = 4 * c; s < 4 * c + 4; ++s)
-                  mma_ts(tOi, tSi + s * 8, vlo + s * (2048 >> 4), ID_PV, s > 0 ? 1u : static_cast<uint32_t>(begun));
-                if (c == 1) tc5::mma_commit(vbar);
-                if (c == 1 && k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
-              }
-              __syncwarp();
-            }
-            if (!run) break;
-            ++pc;
-            begun = true;
-          } else if (lane == 0) {
-            tc5::mbar_arrive(vbar);
+              for (int x = 0; x < HALVES; ++x)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + j * 16), "r"(0) : "memory");
+            tc5::fence_async_smem();
+            __syncwarp();
           }
         }
+        const uint32_t klo = desc_lo(sm + S::RING + st * S::STAGE, DESC_LO_K), kbar = empty + 8 * st;
         if (k < it.k1) {
-          const uint32_t klo = desc_lo(sm + S::RING + st * S::STAGE, DESC_LO_K), kbar = empty + 8 * st;
           if (!(run = k16_wait(full + 8 * st, ph))) break;
           if (++st == STAGES) st = 0, ph ^= 1;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {                          // halves of 64 keys
+          if (was && !(run = k16_wait(pf + 8 * c, pc & 1))) break;
           tc5::fence_after_sync();
-          if (now) {
-            if (tc5::elect_one()) {
+          if (tc5::elect_one()) {
+            if (was) {
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                mma_ts(tOi, tSi + 64 * c + s * 8, vlo + (4 * c + s) * (2048 >> 4), ID_PV, s + c > 0 ? 1u : static_cast<uint32_t>(begun));
+              tc5::mma_commit(pvdone + 8 * i);
+              if (c == 1 && k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
+            }
+            if (now) {
 #pragma unroll
               for (int s = 0; s < D / 16; ++s)
-                mma_ss(tSi, qlo + (((s >> 2) * 128 * 128 + (s & 3) * 32) >> 4), klo + (((s >> 2) * BN * 128 + (s & 3) * 32) >> 4), ID_QK, s > 0);
-              tc5::mma_commit(sfull + 8 * i);
-              tc5::mma_commit(kbar);
-              if (k == it.k1 - 1) tc5::mma_commit(qempty);
+                mma_ss(tSi + 64 * c, qlo + (((s >> 2) * 128 * 128 + (s & 3) * 32) >> 4),
+                       klo + (((s >> 2) * BN * 128 + c * 64 * 128 + (s & 3) * 32) >> 4), ID_QK, s > 0);
+              tc5::mma_commit(sfull + 16 * i + 8 * c);
             }
-            __syncwarp();
-          } else if (lane == 0) {
-            tc5::mbar_arrive(kbar);
+            if (c == 1) {
+              if (k > it.k0) {
+                if (was) tc5::mma_commit(vbar);
+                else tc5::mbar_arrive(vbar);
+              }
+              if (k < it.k1) {
+                if (now) tc5::mma_commit(kbar);
+                else tc5::mbar_arrive(kbar);
+              }
+              if (k == it.k1 - 1) tc5::mma_commit(qempty);     // after this tile's last product with Q, whichever it was
+            }
           }
-          if (!now && k == it.k1 - 1) {                        // (this tile's last product was an earlier block's)
-            if (tc5::elect_one()) tc5::mma_commit(qempty);
-            __syncwarp();
-          }
+          __syncwarp();
         }
+        if (!run) break;
+        if (was) ++pc, begun = true;
         was = now, kbv = kb;
       }
     }
@@ -452,6 +477,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     const uint32_t ts = tS + i * 128 + lanes, to = tO + i * 128 + lanes;
     const float qs = fmaxf(fabsf(a.qscale), 1e-37f);           // a scale of 0: all scores alike, and -inf * qs stays -inf
     constexpr float BIAS = DT == 1 ? 6.f : 0.f;                // fp16 weights are carried times 2^6: their steps below 2^-14 are absolute
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(2 * a.o_ts)) & 31) == 0;
     int syncs = 0;
     const auto tile_sync = [&]() {                             // the softmax warps of a tile (bounded, unlike a named barrier)
       __syncwarp();
@@ -475,73 +501,70 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       for (int k = it.k0; k < it.k1; ++k) {
         const int kb = it.block(k) * BN;
         if (!t.needs(kb)) continue;
-        if (!(run = k16_wait(sfull + 8 * i, sc & 1))) break;
-        ++sc;
-        tc5::fence_after_sync();
-        uint32_t v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc5::tmem_ld32(ts + 32 * c, v[c]);
-        tc5::tmem_ld_wait();
-        if (__builtin_expect(!t.whole(kb), 0)) {
-          const int hi = pos + 1 - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : 0, sk = a.sinks - kb;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t see = low_bits(hi - 32 * c) & (~low_bits(lo - 32 * c) | low_bits(sk - 32 * c));
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(see & (1u << e))) v[c][e] = 0xFF800000u;
-          }
-        }
-        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          m0 = max3(m0, __uint_as_float(v[0][c]), __uint_as_float(v[0][c + 1]));
-          m1 = max3(m1, __uint_as_float(v[1][c]), __uint_as_float(v[1][c + 1]));
-          m2 = max3(m2, __uint_as_float(v[2][c]), __uint_as_float(v[2][c + 1]));
-          m3 = max3(m3, __uint_as_float(v[3][c]), __uint_as_float(v[3][c + 1]));
-        }
-        const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
-        if (__builtin_expect(__any_sync(~0u, m > ref + LAZY), 0)) {
-          const float nr = fmaxf(m, ref), f = ref == -INFINITY ? 0.f : ex2(ref - nr);
-          // S(k) is complete, so every product into O before it is; the next one waits for this P
-          const bool some = l > SEEN;
-          l *= f;
-          if (__any_sync(~0u, some)) {
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tc5::tmem_ld32(to + 32 * c, o);
-              tc5::tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc5::tmem_st32(to + 32 * c, o);
-            }
-          }
-          ref = nr;
-        }
-        const float off = (ref == -INFINITY ? 0.f : -ref) + BIAS;
-        const uint64_t q2 = pk(qs, qs), off2 = pk(off, off);
-        uint64_t sum[4] = {0, 0, 0, 0};
+        const bool whole = t.whole(kb);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (!(run = k16_wait(sfull + 16 * i + 8 * c, sc & 1))) break;
+          tc5::fence_after_sync();
+          uint32_t v[2][32];
+          tc5::tmem_ld32(ts + 64 * c, v[0]);
+          tc5::tmem_ld32(ts + 64 * c + 32, v[1]);
+          ld_wait(v[0]);
+          ld_wait(v[1]);
+          if (__builtin_expect(!whole, 0)) {
+            const int kh = kb + 64 * c, hi = pos + 1 - kh, lo = a.window > 0 ? pos - a.window + 1 - kh : 0, sk = a.sinks - kh;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) hide(v[d], low_bits(hi - 32 * d) & (~low_bits(lo - 32 * d) | low_bits(sk - 32 * d)));
+          }
+          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            m0 = max3(m0, __uint_as_float(v[0][e]), __uint_as_float(v[0][e + 1]));
+            m1 = max3(m1, __uint_as_float(v[0][e + 2]), __uint_as_float(v[0][e + 3]));
+            m2 = max3(m2, __uint_as_float(v[1][e]), __uint_as_float(v[1][e + 1]));
+            m3 = max3(m3, __uint_as_float(v[1][e + 2]), __uint_as_float(v[1][e + 3]));
+          }
+          const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
+          if (__builtin_expect(__any_sync(~0u, m > ref + LAZY), 0)) {
+            const float nr = fmaxf(m, ref), f = ref == -INFINITY ? 0.f : ex2(ref - nr);
+            const bool some = l > SEEN;
+            l *= f;
+            ref = nr;
+            if (__any_sync(~0u, some)) {                       // O holds the products of every earlier half; the next ones wait for this P
+              if (!(run = k16_wait(pvdone + 8 * i, (2 * sc + c - 1) & 1))) break;
+              tc5::fence_after_sync();
+#pragma unroll 1
+              for (int d = 0; d < D / 32; ++d) {
+                uint32_t o[32];
+                tc5::tmem_ld32(to + 32 * d, o);
+                tc5::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc5::tmem_st32(to + 32 * d, o);
+              }
+            }
+          }
+          const float off = (ref == -INFINITY ? 0.f : -ref) + BIAS;
+          const uint64_t q2 = pk(qs, qs), off2 = pk(off, off);
+          uint64_t sum[4] = {0, 0, 0, 0};
           uint32_t p[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const int x = 64 * c + 2 * e;
-            const uint64_t y2 = fma2(pk(__uint_as_float(v[x >> 5][x & 31]), __uint_as_float(v[x >> 5][(x & 31) + 1])), q2, off2);
-            const float2 y = un(y2);
+            const float2 y = un(fma2(pk(__uint_as_float(v[e >> 4][2 * (e & 15)]), __uint_as_float(v[e >> 4][2 * (e & 15) + 1])), q2, off2));
             const float p0 = ex2(y.x), p1 = ex2(y.y);
             sum[e & 3] = add2(sum[e & 3], pk(p0, p1));
             p[e] = Elem<DT>::pack(p0, p1);
           }
-          tc5::tmem_st32(ts + 32 * c, p);
+          tc5::tmem_st32(ts + 64 * c, p);                      // over scores that have been read
+          const float2 l2 = un(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+          l += l2.x + l2.y;
           tc5::tmem_st_wait();
           tc5::fence_before_sync();
           __syncwarp();
-          if (lane == 0) tc5::mbar_arrive(pfull + 16 * i + 8 * c);   // half of P: its products may begin
+          if (lane == 0) tc5::mbar_arrive(pfull + 16 * i + 8 * c);
         }
-        const float2 l2 = un(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-        l += l2.x + l2.y;
+        if (!run) break;
+        ++sc;
       }
       if (!run) break;
       if (l < SEEN) l = 0.f;
@@ -563,7 +586,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           }
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) put8<DT>(out + 32 * c + e, f4(o + e), f4(o + e + 4), inv, any && inv != 0.f);
+            for (int e = 0; e < 32; e += 16)
+              put16<DT>(out + 32 * c + e, f4(o + e), f4(o + e + 4), f4(o + e + 8), f4(o + e + 12), inv, any && inv != 0.f, wide);
           }
           __syncwarp();
         }
@@ -605,27 +629,34 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           }
           const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
 #pragma unroll 1
-          for (int c = 0; c < D / 4; c += 8) {
-            float4 acc[8];
+          for (int c = 0; c < D / 4; c += 4) {                 // 16 dims of four pieces in flight
+            float4 acc[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s = 0; s < it.ns; ++s) {
-              const float2 e2 = __ldcg(ml + static_cast<long long>(s * it.stride) * 256);
-              if (e2.y == 0.f) continue;
-              const float f = ex2(e2.x - M);
-              const float4* q = pq + static_cast<long long>(s * it.stride) * (2 * (D / 4) * 128) + c * 128;
+            for (int e = 0; e < 4; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < it.ns; s += 4) {
+              float4 x[4][4];
+              float f[4];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 x = __ldcg(q + e * 128);
-                acc[e].x = fmaf(f, x.x, acc[e].x);
-                acc[e].y = fmaf(f, x.y, acc[e].y);
-                acc[e].z = fmaf(f, x.z, acc[e].z);
-                acc[e].w = fmaf(f, x.w, acc[e].w);
+              for (int q = 0; q < 4; ++q) {
+                const bool in = s + q < it.ns;
+                const float2 e2 = in ? __ldcg(ml + static_cast<long long>((s + q) * it.stride) * 256) : make_float2(0.f, 0.f);
+                const bool use = in && e2.y != 0.f;            // (0: the piece has no key that this row sees)
+                f[q] = use ? ex2(e2.x - M) : 0.f;
+                const float4* src = pq + static_cast<long long>((s + q) * it.stride) * (2 * (D / 4) * 128) + c * 128;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[q][e] = use ? __ldcg(src + e * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
               }
-            }
-            if (live)
 #pragma unroll
-              for (int e = 0; e < 8; e += 2) put8<DT>(out + 4 * (c + e), acc[e], acc[e + 1], inv, inv != 0.f);
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  acc[e].x = fmaf(f[q], x[q][e].x, acc[e].x);
+                  acc[e].y = fmaf(f[q], x[q][e].y, acc[e].y);
+                  acc[e].z = fmaf(f[q], x[q][e].z, acc[e].z);
+                  acc[e].w = fmaf(f[q], x[q][e].w, acc[e].w);
+                }
+            }
+            if (live) put16<DT>(out + 4 * c, acc[0], acc[1], acc[2], acc[3], inv, inv != 0.f, wide);
           }
           __syncwarp();
         }
