@@ -23,7 +23,8 @@
 namespace k16 {
 namespace {
 
-constexpr int BN = 128;                  // keys per block
+constexpr int BN = 128;                  // keys per block, fetched together
+constexpr int HN = 64;                   // keys per half block, the unit of S, P and the softmax
 constexpr int THREADS = 384;            // three warpgroups: two of softmax, one of MMA (a warp per tile), copies and an idle warp
 constexpr int W_MMA = 8, W_TMA = 10;
 constexpr int REGS_SOFT = 216, REGS_REST = 72;   // 256 x 216 + 128 x 72 = 384 x 168, what the launch has
@@ -48,17 +49,18 @@ struct Item {
 };
 // the tokens of one tile, as positions [pa, pb]
 struct Tile {
-  int pa, pb, last, window, sinks;       // last: index of the last block that the tile needs (-1: none)
+  int pa, pb, last, window, sinks;       // last: the last half block that the tile needs (2 k + half; -1: none)
   FR_DEVI Tile(const Item& it, int i, int tpt, int window_, int sinks_) : last(-1), window(window_), sinks(sinks_) {
     pa = it.pos0 + i * tpt;
     pb = min(it.pos0 + it.tok1 - it.tok0, pa + tpt) - 1;
     if (pb >= max(pa, 0))
-      for (int k = it.k1 - 1; k >= it.k0 && last < 0; --k)
-        if (needs(it.block(k) * BN)) last = k;
+      for (int k = 2 * it.k1 - 1; k >= 2 * it.k0 && last < 0; --k)
+        if (needs(it.block(k >> 1) * BN + (k & 1) * HN)) last = k;
     if (last < 0) pb = -1;                                     // nothing in this item's blocks
   }
-  FR_DEVI bool needs(int kb) const { return kb <= pb && (window <= 0 || kb + BN > pa - window + 1 || kb < sinks); }
-  FR_DEVI bool whole(int kb) const { return kb + BN - 1 <= pa && (window <= 0 || kb > pb - window || kb + BN <= sinks); }
+  // whether a query of the tile sees any of the HN keys from kh on, and whether all of them see them all
+  FR_DEVI bool needs(int kh) const { return kh <= pb && (window <= 0 || kh + HN > pa - window + 1 || kh < sinks); }
+  FR_DEVI bool whole(int kh) const { return kh + HN - 1 <= pa && (window <= 0 || kh > pb - window || kh + HN <= sinks); }
 };
 
 template <int D> struct Smem {
@@ -389,11 +391,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
     if (*abort && lane == 0 && qc) tc5::mbar_wait(qfull, (qc - 1) & 1);
   } else if (w == W_MMA || w == W_MMA + 1) {                   // ------------------------------------- MMAs, a warp per tile
     // the softmax takes |qscale|: a negative scale negates the A operand
-    const uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, 64) | (a.qscale < 0.f ? A_NEGATE : 0u);
+    const uint32_t ID_QK = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, HN) | (a.qscale < 0.f ? A_NEGATE : 0u);
     constexpr uint32_t ID_PV = tc5::idesc(1, DT == 0 ? 1 : 0, DT == 0 ? 1 : 0, 128, D) | B_MN_MAJOR;
     const int i = w - W_MMA;
     const uint32_t tSi = tS + i * 128, tOi = tO + i * 128, qlo = desc_lo(sm + i * S::QT, DESC_LO_K), pf = pfull + 16 * i;
-    int qc = 0, pc = 0;                                        // query pairs and P tiles consumed
+    int qc = 0, pc0 = 0, pc1 = 0;                              // query pairs and P halves consumed
     int st = 0, ph = 0;                                        // the ring's next tile: K(k0), V(k0), K(k0 + 1), ... of every item
     bool run = true;
     for (int ic = 0; run; ++ic) {
@@ -408,17 +410,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (!k16_wait(qfull, qc & 1)) break;
       ++qc;
       tc5::fence_after_sync();
-      bool was = false, begun = false;                         // the tile needs V(k - 1); its O has begun
+      int was = 0;                                             // bit c: the tile needs half c of V(k - 1)
+      uint32_t begun = 0;                                      // its O has begun
       int kbv = 0;                                             // first key of block k - 1
       for (int k = it.k0; k <= it.k1; ++k) {
         const int kb = k < it.k1 ? it.block(k) * BN : 0;
-        const bool now = k < it.k1 && t.needs(kb);
+        const int now = k < it.k1 ? (t.needs(kb) ? 1 : 0) | (t.needs(kb + HN) ? 2 : 0) : 0;
         // Every tile of the ring is waited for, needed or not: the parity of a later phase would not tell.
         const uint32_t sv = sm + S::RING + st * S::STAGE, vlo = desc_lo(sv, DESC_LO_MN), vbar = empty + 8 * st;
         if (k > it.k0) {
           if (!(run = k16_wait(full + 8 * st, ph))) break;
           if (++st == STAGES) st = 0, ph ^= 1;
-          if (was && kbv + BN > it.len) {                      // values behind the sequence: 0 * NaN would be NaN
+          if (was && kbv + BN > it.len) {       // values behind the sequence: 0 * NaN would be NaN
             for (int j = (it.len - kbv) * 8 + lane; j < BN * 8; j += 32)
 #pragma unroll
               for (int x = 0; x < HALVES; ++x)
@@ -433,40 +436,34 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           if (++st == STAGES) st = 0, ph ^= 1;
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {                          // halves of 64 keys
-          if (was && !(run = k16_wait(pf + 8 * c, pc & 1))) break;
+        for (int c = 0; c < 2; ++c) {
+          if ((was >> c & 1) && !(run = k16_wait(pf + 8 * c, (c ? pc1 : pc0) & 1))) break;
           tc5::fence_after_sync();
           if (tc5::elect_one()) {
-            if (was) {
+            if (was >> c & 1) {
 #pragma unroll
-              for (int s = 0; s < 4; ++s)
-                mma_ts(tOi, tSi + 64 * c + s * 8, vlo + (4 * c + s) * (2048 >> 4), ID_PV, s + c > 0 ? 1u : static_cast<uint32_t>(begun));
+              for (int s = 0; s < HN / 16; ++s)
+                mma_ts(tOi, tSi + HN * c + s * 8, vlo + (4 * c + s) * (2048 >> 4), ID_PV, s > 0 ? 1u : begun);
               tc5::mma_commit(pvdone + 8 * i);
-              if (c == 1 && k - 1 == t.last) tc5::mma_commit(ofull + 8 * i);
+              if (2 * (k - 1) + c == t.last) tc5::mma_commit(ofull + 8 * i);
             }
-            if (now) {
+            if (now >> c & 1) {
 #pragma unroll
               for (int s = 0; s < D / 16; ++s)
-                mma_ss(tSi + 64 * c, qlo + (((s >> 2) * 128 * 128 + (s & 3) * 32) >> 4),
-                       klo + (((s >> 2) * BN * 128 + c * 64 * 128 + (s & 3) * 32) >> 4), ID_QK, s > 0);
+                mma_ss(tSi + HN * c, qlo + (((s >> 2) * 128 * 128 + (s & 3) * 32) >> 4),
+                       klo + (((s >> 2) * BN * 128 + c * HN * 128 + (s & 3) * 32) >> 4), ID_QK, s > 0);
               tc5::mma_commit(sfull + 16 * i + 8 * c);
             }
-            if (c == 1) {
-              if (k > it.k0) {
-                if (was) tc5::mma_commit(vbar);
-                else tc5::mbar_arrive(vbar);
-              }
-              if (k < it.k1) {
-                if (now) tc5::mma_commit(kbar);
-                else tc5::mbar_arrive(kbar);
-              }
+            if (c == 1) {                                      // (a commit without products before it arrives at once)
+              if (k > it.k0) tc5::mma_commit(vbar);
+              if (k < it.k1) tc5::mma_commit(kbar);
               if (k == it.k1 - 1) tc5::mma_commit(qempty);     // after this tile's last product with Q, whichever it was
             }
           }
           __syncwarp();
+          if (was >> c & 1) begun = 1, c ? ++pc1 : ++pc0;
         }
         if (!run) break;
-        if (was) ++pc, begun = true;
         was = now, kbv = kb;
       }
     }
@@ -484,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (lane == 0) tc5::mbar_arrive(tsync + 8 * i);
       return k16_wait(tsync + 8 * i, syncs++ & 1);
     };
-    int sc = 0, oc = 0;                                        // S and O tiles consumed
+    int sc[2] = {0, 0}, oc = 0;                                // S halves and O tiles consumed
     bool run = true;
     for (int ic = 0; run; ++ic) {
       const int sl = ic & 1;
@@ -500,19 +497,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       float ref = -INFINITY, l = 0.f;
       for (int k = it.k0; k < it.k1; ++k) {
         const int kb = it.block(k) * BN;
-        if (!t.needs(kb)) continue;
-        const bool whole = t.whole(kb);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (!(run = k16_wait(sfull + 16 * i + 8 * c, sc & 1))) break;
+          const int kh = kb + HN * c;
+          if (!t.needs(kh)) continue;
+          const bool whole = t.whole(kh);
+          if (!(run = k16_wait(sfull + 16 * i + 8 * c, sc[c] & 1))) break;
+          ++sc[c];
           tc5::fence_after_sync();
           uint32_t v[2][32];
-          tc5::tmem_ld32(ts + 64 * c, v[0]);
-          tc5::tmem_ld32(ts + 64 * c + 32, v[1]);
+          tc5::tmem_ld32(ts + HN * c, v[0]);
+          tc5::tmem_ld32(ts + HN * c + 32, v[1]);
           ld_wait(v[0]);
           ld_wait(v[1]);
           if (__builtin_expect(!whole, 0)) {
-            const int kh = kb + 64 * c, hi = pos + 1 - kh, lo = a.window > 0 ? pos - a.window + 1 - kh : 0, sk = a.sinks - kh;
+            const int hi = pos + 1 - kh, lo = a.window > 0 ? pos - a.window + 1 - kh : 0, sk = a.sinks - kh;
 #pragma unroll
             for (int d = 0; d < 2; ++d) hide(v[d], low_bits(hi - 32 * d) & (~low_bits(lo - 32 * d) | low_bits(sk - 32 * d)));
           }
@@ -531,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
             l *= f;
             ref = nr;
             if (__any_sync(~0u, some)) {                       // O holds the products of every earlier half; the next ones wait for this P
-              if (!(run = k16_wait(pvdone + 8 * i, (2 * sc + c - 1) & 1))) break;
+              if (!(run = k16_wait(pvdone + 8 * i, (sc[0] + sc[1]) & 1))) break;
               tc5::fence_after_sync();
 #pragma unroll 1
               for (int d = 0; d < D / 32; ++d) {
@@ -555,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
             sum[e & 3] = add2(sum[e & 3], pk(p0, p1));
             p[e] = Elem<DT>::pack(p0, p1);
           }
-          tc5::tmem_st32(ts + 64 * c, p);                      // over scores that have been read
+          tc5::tmem_st32(ts + HN * c, p);                      // over scores that have been read
           const float2 l2 = un(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
           l += l2.x + l2.y;
           tc5::tmem_st_wait();
@@ -564,7 +563,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           if (lane == 0) tc5::mbar_arrive(pfull + 16 * i + 8 * c);
         }
         if (!run) break;
-        ++sc;
       }
       if (!run) break;
       if (l < SEEN) l = 0.f;
