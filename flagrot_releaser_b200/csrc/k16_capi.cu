@@ -99,8 +99,8 @@ int k16_attn(int dtype, const void* q, long long q_bs, const void* pool, long lo
   a.G = G;
   a.D = D;
   a.qscale = qscale;
-  a.window = window;
-  a.sinks = sinks;
+  a.window = window < (1 << 30) ? window : 1 << 30;    // positions are below 2^30
+  a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
   a.weights = weights;
   a.w_bs = w_bs;
   a.w_hs = w_hs;
@@ -132,8 +132,8 @@ int k16_prefill(int dtype, const void* q, long long q_ts, int T, const int* cu_q
   a.G = G;
   a.D = D;
   a.qscale = qscale;
-  a.window = window;
-  a.sinks = sinks;
+  a.window = window < (1 << 30) ? window : 1 << 30;    // positions are below 2^30
+  a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
   a.tickets = tickets;
   a.ws = static_cast<unsigned char*>(ws);
   a.out = out;

@@ -30,9 +30,8 @@ constexpr int W_MMA = 8, W_TMA = 10;
 constexpr int REGS_SOFT = 216, REGS_REST = 72;   // 256 x 216 + 128 x 72 = 384 x 168, what the launch has
 constexpr int MAX_HEADS = 128;           // q heads per item
 constexpr float LAZY = 8.f;
-constexpr float SEEN = 1e-20f;           // a row that has seen a key has a sum of about 1 at least
 constexpr int MAX_SPLIT = 32;            // pieces of a pair's key blocks
-constexpr int SLOTS = 4 * 148;           // workspace slots: pieces of split pairs
+constexpr int SLOTS = 4 * 148;           // workspace slots at most: pieces of split pairs
 constexpr int SPLIT_COST = 4;            // what a piece costs besides its blocks, in blocks
 
 __device__ int g_status;
@@ -178,7 +177,8 @@ template <int DT> FR_DEVI void put16(uint16_t* out, float4 x, float4 y, float4 z
 
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ PrefillArgs a, const __grid_constant__ CUtensorMap qmap,
-                                                        const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows) {
+                                                        const __grid_constant__ CUtensorMap kvmap, int hb, int nhg, int box_rows,
+                                                        int slots) {
   using S = Smem<D>;
   constexpr int STAGES = S::STAGES, HALVES = D / 64;
   extern __shared__ unsigned char smem_raw[];
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       const int sp = lane + 1;                                 // lane i: i + 1 pieces
       const float avg = all / static_cast<float>(pairs), n = ceilf(fminf(avg, static_cast<float>(sp)));
       float cost = ceilf(rest * n / gridDim.x) * (avg / n + (sp > 1 ? SPLIT_COST : 0));
-      if (rest * sp > SLOTS || avg < 1.f) cost = sp == 1 ? 1e30f : INFINITY;
+      if (rest * sp > slots || avg < 1.f) cost = sp == 1 ? 1e30f : INFINITY;
       float best = cost;
 #pragma unroll
       for (int d = 16; d; d >>= 1) best = fminf(best, __shfl_xor_sync(~0u, best, d));
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
           const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * qs;
           if (__builtin_expect(__any_sync(~0u, m > ref + LAZY), 0)) {
             const float nr = fmaxf(m, ref), f = ref == -INFINITY ? 0.f : ex2(ref - nr);
-            const bool some = l > SEEN;
+            const bool some = l > 0.f;                         // (a row that has seen a key has a sum of about 1 at least)
             l *= f;
             ref = nr;
             if (__any_sync(~0u, some)) {                       // O holds the products of every earlier half; the next ones wait for this P
@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         if (!run) break;
       }
       if (!run) break;
-      if (l < SEEN) l = 0.f;
       const bool any = t.last >= 0;
       if (any) {
         if (!(run = k16_wait(ofull + 8 * i, oc & 1))) break;
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         // this piece's sums to its slot, [dims / 4][row] x 16 bytes; the last piece of the tile to arrive joins them in order
         const int rr = i * (D / 4) * 128 + r;
         float4* po = reinterpret_cast<float4*>(a.ws) + static_cast<long long>(it.slot) * (2 * (D / 4) * 128) + rr;
-        float2* pl = reinterpret_cast<float2*>(a.ws + static_cast<long long>(SLOTS) * (2 * D * 128 * 4));
+        float2* pl = reinterpret_cast<float2*>(a.ws + static_cast<long long>(slots) * (2 * D * 128 * 4));
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           if (any) {
@@ -672,11 +671,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
 }
 
 template <int DT, int D>
-cudaError_t launch_p(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int dev, int grid, cudaStream_t st) {
+cudaError_t launch_p(const PrefillArgs& a, const CUtensorMap& qm, const CUtensorMap& kv, int hb, int nhg, int box, int slots, int dev, int grid, cudaStream_t st) {
   const auto k = k_prefill<DT, D>;
   static std::atomic<bool> done[MAX_DEVICES];
   if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, qm, kv, hb, nhg, box);
+  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, qm, kv, hb, nhg, box, slots);
 }
 
 }  // namespace
@@ -692,9 +691,15 @@ static long long max_pairs(int rows, int Hkv, int G, long long new_tokens) {
   groups(G, nhg, hb, tpt);
   return (new_tokens / (2 * tpt) + rows) * Hkv * nhg;
 }
-// sums and (reference, denominator) of every slot; a pair is split into MAX_SPLIT pieces at most
-long long prefill_ws_bytes(int, int, int, int D, long long) { return static_cast<long long>(SLOTS) * 256 * (D * 4 + 8); }
-long long prefill_tickets(int, int, int, long long) { return 2 * SLOTS; }
+static int max_slots(int rows, int Hkv, int G, long long new_tokens) {
+  const long long n = max_pairs(rows, Hkv, G, new_tokens) * MAX_SPLIT;
+  return static_cast<int>(n < SLOTS ? n : SLOTS);
+}
+// sums, then (reference, denominator), of every slot
+long long prefill_ws_bytes(int rows, int Hkv, int G, int D, long long new_tokens) {
+  return static_cast<long long>(max_slots(rows, Hkv, G, new_tokens)) * 256 * (D * 4 + 8);
+}
+long long prefill_tickets(int rows, int Hkv, int G, long long new_tokens) { return 2 * max_slots(rows, Hkv, G, new_tokens); }
 
 int prefill_status() {
   int v = -1;
@@ -715,10 +720,10 @@ cudaError_t prefill(int dtype, const PrefillArgs& a, cudaStream_t st) {
     e = encode3(&kv, dtype, a.c.pool, static_cast<uint64_t>((a.c.num_pages * a.c.Hkv * 2) << a.c.page_sh), a.D * 2ull, a.D / 64, 128, box, 1);
   if (e != cudaSuccess) return e;
   const long long items = max_pairs(a.B, a.c.Hkv, a.G, a.T) * MAX_SPLIT;
-  const int grid = static_cast<int>(items < sms ? items : sms);
+  const int grid = static_cast<int>(items < sms ? items : sms), slots = max_slots(a.B, a.c.Hkv, a.G, a.T);
   if (dtype == 0)
-    return a.D == 128 ? launch_p<0, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch_p<0, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
-  return a.D == 128 ? launch_p<1, 128>(a, qm, kv, hb, nhg, box, dev, grid, st) : launch_p<1, 64>(a, qm, kv, hb, nhg, box, dev, grid, st);
+    return a.D == 128 ? launch_p<0, 128>(a, qm, kv, hb, nhg, box, slots, dev, grid, st) : launch_p<0, 64>(a, qm, kv, hb, nhg, box, slots, dev, grid, st);
+  return a.D == 128 ? launch_p<1, 128>(a, qm, kv, hb, nhg, box, slots, dev, grid, st) : launch_p<1, 64>(a, qm, kv, hb, nhg, box, slots, dev, grid, st);
 }
 
 }  // namespace k16

@@ -29,6 +29,7 @@ _PKG = Path(__file__).resolve().parent
 ABI = 1
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 PAGES, HEAD_DIMS = (16, 32, 64, 128), (64, 128)
+MAX_POS = 1 << 30                # positions are below it
 
 
 def _lib_path() -> Path:
@@ -169,6 +170,7 @@ def attn(q, pool, block_table, seq_lens, out, ws, qscale, window=0, sinks=0, wei
         assert wB == B and wH == Hkv and W >= width * page and (w1 == 1 or W <= 1), "weights: fp32 [B, Hkv, >= width * page]"
         _stream(weights)
         wp = weights.data_ptr()
+    window, sinks = min(window, MAX_POS), min(sinks, MAX_POS)
     _check(lib().k16_attn(dt, q.data_ptr(), qs, pool.data_ptr(), npg, block_table.data_ptr(), bs, width, seq_lens.data_ptr(), B, Hkv, G,
                           D, page, qscale, window, sinks, wp, wb, wh, ws.ptickets, ws.ntickets, ws.pbuf, ws.nbytes, out.data_ptr(),
                           os_, stream), "k16_attn")
@@ -190,6 +192,7 @@ def prefill(q, cu_q, pool, block_table, seq_lens, out, qscale, window=0, sinks=0
         return
     assert ws is not None, "ws: a Workspace made with new_tokens"
     stream = _stream(q, cu_q, pool, block_table, seq_lens, out, ws.buf)
+    window, sinks = min(window, MAX_POS), min(sinks, MAX_POS)
     _check(lib().k16_prefill(dt, q.data_ptr(), qs, T, cu_q.data_ptr(), pool.data_ptr(), npg, block_table.data_ptr(), bs, width,
                              seq_lens.data_ptr(), B, Hkv, G, D, page, qscale, window, sinks, ws.ptickets, ws.ntickets, ws.pbuf,
                              ws.nbytes, out.data_ptr(), os_, stream), "k16_prefill")

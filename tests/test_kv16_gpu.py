@@ -220,6 +220,29 @@ def test_attn_offsets_past_32_bits(K):
     assert torch.equal(pool[npg - 1, :, 0, 15], kv[0, :Hkv]) and torch.equal(pool[npg - 2, :, 1, 15], kv[1, Hkv:])
 
 
+@pytest.mark.parametrize("G,Hkv", [(130, 1), (71, 2), (256, 1)])
+def test_attn_many_heads_per_group(K, G, Hkv):
+    g = gen(G)
+    lens = [1, 40, 700]
+    pool, bt, ln = R.make_cache(lens, Hkv, 64, 16, BF, g)
+    q = queries(3, G * Hkv, 64, BF, g)
+    w0 = torch.rand(3, Hkv, bt.shape[1] * 16, generator=g).to(DEV)
+    w1 = w0.clone()
+    out = run_attn(K, q, pool, bt, ln, 0.17, weights=w1)
+    check_attn(out, q, pool, bt, ln, 0.17, 0, 0, w0, w1)
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 40, 2 ** 35), (-7, 5), (5, 2 ** 31 - 1), (0, 3)])
+def test_window_and_sinks_of_any_size(K, window, sinks):
+    """a window or sinks beyond every position act as no window; a negative window is none"""
+    g = gen(13)
+    pool, bt, ln = R.make_cache([300, 17], 1, 64, 16, BF, g)
+    q = queries(2, 4, 64, BF, g)
+    out = run_attn(K, q, pool, bt, ln, 0.2, window, sinks)
+    check_attn(out, q, pool, bt, ln, 0.2, min(window, 1 << 30), min(sinks, 1 << 30))
+    check_prefill(K, [300, 17], [300, 9], 1, 4, 64, 16, BF, window, sinks, 17)
+
+
 def test_attn_workspace_of_a_larger_call_and_refusal(K):
     """one workspace serves smaller calls too, in any order; a call it is too small for is refused"""
     g = gen(7)
@@ -288,6 +311,58 @@ def test_prefill_more_new_tokens_than_cached(K):
     """tokens at negative positions see nothing and give zeros"""
     check_prefill(K, [4, 0, 30], [10, 7, 30], 2, 4, 128, 16, BF, 0, 0, 12)
     check_prefill(K, [4, 0, 30], [10, 7, 30], 2, 4, 64, 16, FP, 3, 1, 13)
+
+
+@pytest.mark.parametrize("G,Hkv", [(128, 1), (130, 1), (65, 2), (200, 1)])
+def test_prefill_many_heads_per_group(K, G, Hkv):
+    check_prefill(K, [150, 9], [20, 9], Hkv, G, 64, 16, BF, 0, 0, 18)
+
+
+def test_prefill_table_entries_outside_the_pool_read_as_zeros(K):
+    g = gen(19)
+    pool, bt, ln = R.make_cache([300], 2, 64, 16, BF, g)
+    q = queries(40, 8, 64, BF, g)
+    bad = bt.clone()
+    bad[0, 3], bad[0, 11] = -1, pool.shape[0] + 5
+    ref = bad.clone()
+    ref[0, 3] = ref[0, 11] = pool.shape[0]
+    ws, cu = K.Workspace(1, 2, 4, 64, bt.shape[1] * 16, DEV, new_tokens=40), torch.tensor([0, 40], dtype=torch.int32, device=DEV)
+    a, b = torch.empty(40, 512, dtype=BF, device=DEV), torch.empty(40, 512, dtype=BF, device=DEV)
+    K.prefill(q, cu, pool, bad, ln, a, 0.2, ws=ws)
+    K.prefill(q, cu, torch.cat([pool, torch.zeros_like(pool[:1])]), ref, ln, b, 0.2, ws=ws)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lens,new,Hkv,G,D", [([33280] * 2, [512, 300], 8, 4, 128), ([8000, 5100], [8000, 5100], 4, 8, 64)])
+def test_prefill_repeated_calls_agree_bit_for_bit(K, lens, new, Hkv, G, D):
+    """split pairs are joined in the order of their pieces, whichever ends last"""
+    g = gen(20)
+    pool, bt, ln = R.make_cache(lens, Hkv, D, 16, BF, g)
+    T = sum(new)
+    q = queries(T, Hkv * G, D, BF, g)
+    cu = torch.tensor([0, new[0], T], dtype=torch.int32, device=DEV)
+    ws = K.Workspace(2, Hkv, G, D, bt.shape[1] * 16, DEV, new_tokens=T)
+    first = None
+    for _ in range(20):
+        out = torch.empty(T, Hkv * G * D, dtype=BF, device=DEV)
+        K.prefill(q, cu, pool, bt, ln, out, 0.12, window=3000 if D == 64 else 0, sinks=4, ws=ws)
+        first = out if first is None else first
+        assert torch.equal(first, out)
+    assert int(ws.tickets.abs().max()) == 0
+
+
+def test_prefill_workspace_is_checked(K):
+    g = gen(21)
+    pool, bt, ln = R.make_cache([100], 1, 64, 16, BF, g)
+    q, cu = queries(100, 4, 64, BF, g), torch.tensor([0, 100], dtype=torch.int32, device=DEV)
+    out = torch.empty(100, 256, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="code -4"):
+        K.prefill(q, cu, pool, bt, ln, out, 0.1, ws=K.Workspace(1, 1, 4, 64, 112, DEV))
+    big = K.Workspace(3, 2, 8, 128, 4096, DEV, weights=True, new_tokens=5000)       # serves smaller calls
+    K.prefill(q, cu, pool, bt, ln, out, 0.1, ws=big)
+    k, v = R.rows_of(pool, bt[0], 100)
+    o, _, A, S = R.attend(q.double(), k, v, torch.arange(100), 0.1, 0, 0)
+    assert bool(((out.view(100, 4, 64).double() - o).abs() <= bound(o, A, S, 64, 100, BF, True)).all())
 
 
 def test_prefill_extreme_scores(K):
@@ -492,6 +567,59 @@ def test_serving_run(K):
 
 def test_serving_run_captured(K):
     serve(K, 8, True)
+
+
+def chain(K, sync):
+    """writes, prompts, decode steps and evictions one after the other, with torch's own kernels between them"""
+    g = gen(51)
+    B, Hkv, G, D, page, width, budget = 4, 2, 4, 128, 16, 12, 64
+    npg = B * width
+    pool = torch.zeros(npg, Hkv, 2, page, D, dtype=BF, device=DEV)
+    bt = torch.randperm(npg, generator=g).int().view(B, width).to(DEV)
+    ws = K.Workspace(B, Hkv, G, D, width * page, DEV, weights=True, new_tokens=B * 90)
+    seen = []
+
+    def done(*t):
+        if sync:
+            torch.cuda.synchronize()
+        seen.extend(x.clone() for x in t)
+
+    for rep in range(6):
+        n = 60 + 5 * rep
+        kv = torch.randn(B * n, 2 * Hkv, D, generator=g).to(BF).to(DEV)
+        q = (torch.randn(B * n, Hkv * G, D, generator=g) * 1.5).to(BF).to(DEV)
+        t = torch.arange(n, device=DEV)
+        slots = (bt[:, t // page].long() * page + t % page).view(-1)
+        cu = torch.arange(B + 1, dtype=torch.int32, device=DEV) * n
+        ln = torch.full((B,), n, dtype=torch.int32, device=DEV)
+        w = torch.zeros(B, Hkv, width * page, device=DEV)
+        out, o1 = torch.empty(B * n, Hkv * G * D, dtype=BF, device=DEV), torch.empty(B, Hkv * G * D, dtype=BF, device=DEV)
+        K.write(kv, slots, pool)
+        K.prefill(q, cu, pool, bt, ln, out, 0.12, ws=ws)
+        done(out)
+        for step in range(8):
+            m = ln.long()
+            K.write(kv[step * B:(step + 1) * B], bt.long().gather(1, (m // page)[:, None])[:, 0] * page + m % page, pool)
+            ln += 1
+            K.attn(q[step * B:(step + 1) * B], pool, bt, ln, o1, ws, 0.12, weights=w)
+            q[(step + 1) * B:(step + 2) * B] += o1.view(B, Hkv * G, D)
+            done(o1, w)
+            if step % 3 == 2:
+                kept = torch.empty(B, Hkv, budget, dtype=torch.int32, device=DEV)
+                nl, nw = torch.empty(B, dtype=torch.int32, device=DEV), torch.empty_like(w)
+                K.evict(pool, bt, ln, w, budget, 2, 16, kept, nl, nw)
+                ln, w = nl, nw
+                done(kept, nl, nw)
+    torch.cuda.synchronize()
+    return seen
+
+
+def test_kernels_launched_early_keep_the_streams_order(K):
+    """the same chain with the host waiting after every call and without any wait: the same bits"""
+    a = chain(K, True)
+    for _ in range(3):
+        b = chain(K, False)
+        assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_side_streams_and_graphs_with_their_own_workspaces(K):
