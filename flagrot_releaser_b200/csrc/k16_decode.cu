@@ -43,14 +43,14 @@ template <int D> struct Smem {
   static constexpr int MERGE = STAGES * STAGE;                 // float [NW][8][D]
   static constexpr int ML = MERGE + NW * 8 * D * 4;            // float2 [NW][8]
   static constexpr int BAR = ML + NW * 8 * 8;                  // full[STAGES], empty[STAGES]
-  static constexpr int RED = BAR + 2 * STAGES * 8;             // long long [NW + 1]; abort flag; last-arriver flag
-  static constexpr int TOTAL = RED + 64 + 1024;                // slack: the ring starts on a 1024-byte boundary
+  static constexpr int RED = BAR + 2 * STAGES * 8;             // long long [NW + 1]; int [2 (NW + 1)]; abort flag; last-arriver flag
+  static constexpr int TOTAL = RED + 96 + 1024;                // slack: the ring starts on a 1024-byte boundary
 };
 
 // a row's visible keys as blocks: [0, nsb) cover the sinks, the others start at block wb
 struct Row {
-  int len, s1, lo, nsb, wb, nblk, nv;
-  FR_DEVI void set(int len_, int window, int sinks) {
+  int len, s1, lo, nsb, wb, nblk, nv;    // nv: its room in the list
+  FR_DEVI void set(int len_, int window, int sinks, int pad) {
     len = len_;
     const Span sp(len - 1, window, sinks);
     s1 = sp.s1;
@@ -58,7 +58,7 @@ struct Row {
     wb = lo / BLK;
     nsb = min((s1 + BLK - 1) / BLK, wb);
     nblk = len > 0 ? nsb + (len + BLK - 1) / BLK - wb : 0;
-    nv = (nblk + 3) & ~3;
+    nv = nblk > 0 ? max((nblk + 3) & ~3, pad) : 0;
   }
   FR_DEVI int block(int k) const { return k < nsb ? k : wb + k - nsb; }
   FR_DEVI bool visible(int j) const { return j < len && (j < s1 || j >= lo); }
@@ -69,12 +69,13 @@ struct Row {
 // the pieces of a CTA's range, in order; every warp walks them for itself
 struct Walk {
   const AttnArgs& a;
-  int Hv, b;
+  int Hv, pad, b;
   long long f, fend, row0, quota;
   Row r;
   int seg, k0, k1;                       // piece: blocks [k0, k1) of segment seg (kv head, head group) of row b
   long long f0;                          // where the segment begins
-  FR_DEVI Walk(const AttnArgs& a_, int Hv_, long long quota_, long long begin, long long total) : a(a_), Hv(Hv_), quota(quota_) {
+  FR_DEVI Walk(const AttnArgs& a_, int Hv_, int pad_, long long quota_, long long begin, long long total)
+      : a(a_), Hv(Hv_), pad(pad_), quota(quota_) {
     f = begin;
     fend = min(begin + quota, total);
     row0 = 0;
@@ -85,7 +86,7 @@ struct Walk {
       long long n = 0;
       if (r0 + lane < a.B) {
         Row x;
-        x.set(a.c.len(r0 + lane), a.window, a.sinks);
+        x.set(a.c.len(r0 + lane), a.window, a.sinks, pad);
         n = static_cast<long long>(x.nv) * Hv;
       }
       long long s = n;
@@ -103,13 +104,13 @@ struct Walk {
       }
       row0 += __shfl_sync(~0u, s, 31);
     }
-    r.set(a.c.len(b), a.window, a.sinks);
+    r.set(a.c.len(b), a.window, a.sinks, pad);
   }
   FR_DEVI bool next() {
     while (f < fend) {
       while (f - row0 >= static_cast<long long>(r.nv) * Hv) {
         row0 += static_cast<long long>(r.nv) * Hv;
-        r.set(a.c.len(++b), a.window, a.sinks);
+        r.set(a.c.len(++b), a.window, a.sinks, pad);
       }
       const long long off = f - row0;
       seg = static_cast<int>(off / r.nv);
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
   unsigned char* base = smem_raw + (sm - raw);
   const uint32_t full = sm + S::BAR, empty = full + 8 * STAGES;
   long long* red = reinterpret_cast<long long*>(base + S::RED);
-  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(base + S::RED + 48);
+  int* redm = reinterpret_cast<int*>(base + S::RED + 40);
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(base + S::RED + 80);
   volatile uint32_t* flag = abort + 1;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int Hv = a.c.Hkv * nhg, Hq = a.c.Hkv * a.G;
@@ -253,23 +255,38 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
   after_previous();
   // the list's length; rows that see nothing are written as zeros here
   long long total = 0;
+  int most = 0, rows = 0;                                      // the longest segment; rows that see something
   for (int b = tid; b < a.B; b += THREADS) {
     Row r;
-    r.set(a.c.len(b), a.window, a.sinks);
-    total += static_cast<long long>(r.nv) * Hv;
+    r.set(a.c.len(b), a.window, a.sinks, 0);
+    total += r.nv;
+    most = max(most, r.nv);
+    rows += r.nv > 0;
   }
-  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-  if (lane == 0) red[w] = total;
+  total = (static_cast<long long>(__reduce_add_sync(~0u, static_cast<unsigned>(total >> 20))) << 20) +
+          __reduce_add_sync(~0u, static_cast<unsigned>(total & 0xFFFFF));
+  most = __reduce_max_sync(~0u, most);
+  rows = __reduce_add_sync(~0u, rows);
+  if (lane == 0) red[w] = total, redm[2 * w] = most, redm[2 * w + 1] = rows;
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
     if (a.c.len(b) == 0)
       for (int i = tid; i < Hq * D / 2; i += THREADS)
         reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + b * a.o_bs)[i] = 0;
   __syncthreads();
-  total = 0;
+  total = rows = 0;
 #pragma unroll
-  for (int i = 0; i <= NW; ++i) total += red[i];
-  const long long quota = max(((total + gridDim.x - 1) / gridDim.x + 3) & ~3ll, 4ll);
-  Walk wk(a, Hv, quota, static_cast<long long>(blockIdx.x) * quota, total);
+  for (int i = 0; i <= NW; ++i) total += red[i], most = max(most, redm[2 * i]), rows += redm[2 * i + 1];
+  total *= Hv;
+  long long quota = max(((total + gridDim.x - 1) / gridDim.x + 3) & ~3ll, 4ll);
+  int pad = 0;
+  // No more segments than CTAs and none much longer than a range: a whole segment each, and nothing to join (32 rows x 8 heads
+  // x 1028 visible keys: 34.4 -> 29.4 us; where it does not hold the ranges stay equal).
+  if (static_cast<long long>(rows) * Hv <= gridDim.x && 4 * most <= 5 * quota) {
+    pad = most;
+    quota = max(most, 4);
+    total = static_cast<long long>(rows) * Hv * most;
+  }
+  Walk wk(a, Hv, pad, quota, static_cast<long long>(blockIdx.x) * quota, total);
 
   // where a block's 16-key half, dim half and values are in a stage: pages of 16 tokens come as [dim half][16 keys | 16 values]
   // per page, larger ones as [dim half][32 keys] and the same of values
