@@ -539,7 +539,7 @@ cudaError_t launch_d(const AttnArgs& a, const CUtensorMap& map, int dev, int gri
   const auto k = k_decode<DT, D, NT>;
   static std::atomic<bool> done[MAX_DEVICES];
   if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, map, nhg, part, lse, scores, ld);
+  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, st, a, map, nhg, part, lse, scores, ld);
 }
 template <int DT, int D>
 cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
@@ -584,7 +584,7 @@ cudaError_t attn(int dtype, const AttnArgs& a, cudaStream_t st) {
   const long long chunks = (width + 1023) / 1024;
   if (chunks * a.B * a.c.Hkv > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   const bool vec = (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0 && a.w_bs % 4 == 0 && a.w_hs % 4 == 0;
-  return launch(vec ? k_weights<true> : k_weights<false>, static_cast<unsigned>(chunks * a.B * a.c.Hkv), 256, 0, 0, true, st, a,
+  return launch(vec ? k_weights<true> : k_weights<false>, static_cast<unsigned>(chunks * a.B * a.c.Hkv), 256, 0, 0, st, a,
                 static_cast<const float*>(scores), ld, static_cast<const float*>(lse), static_cast<int>(chunks));
 }
 

@@ -2,8 +2,8 @@
 //
 // HBM bound: 8 D bytes move per kept (token, kv head) (key and value row, read and written), 4 bytes are read per weight.
 // Two launches:
-//   k_select  a cluster of 1 to 8 CTAs per (row, kv head): the threshold by a radix search over order-preserving keys (11, 11
-//             and 10 bits; the CTAs' histograms are added through distributed shared memory), then one scan that writes the
+//   k_select  a cluster of 1 to 8 CTAs per (row, kv head): the threshold by a radix search over order-preserving keys (four
+//             digits of 8 bits; the CTAs' histograms are added through distributed shared memory), then one scan that writes the
 //             kept positions and their weights;
 //   k_copy    (other pages) a CTA per 64 kept tokens, or
 //   k_move    (in place) a cluster per (row, kv head) that moves the rows down step by step: a kept token only moves to a lower
@@ -19,7 +19,7 @@ namespace k16 {
 namespace {
 
 constexpr int NT = 512, NWARP = NT / 32;
-constexpr int BINS = 2048;
+constexpr int DIGIT = 8, BINS = 1 << DIGIT, PASSES = 32 / DIGIT;
 constexpr int MAX_KEYS = 16384;                       // keys of a CTA's positions that shared memory holds
 
 // order-preserving key of a weight: a > b as floats iff key(a) > key(b); -0 equals +0, NaN is below everything
@@ -51,8 +51,8 @@ FR_DEVI int block_scan(int v, int* red) {
 // CL: the cluster has more than one CTA.
 template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
   extern __shared__ float sw[];
-  __shared__ int hist[3][BINS];
-  __shared__ int red[NWARP], s_sure[NWARP], s_ties[NWARP], s_slice[3];
+  __shared__ int hist[PASSES][BINS];
+  __shared__ int red[NWARP], s_sure[NWARP], s_ties[NWARP];
   __shared__ uint32_t s_digit;
   __shared__ int s_left;
   __shared__ int s_count[2];                          // this CTA's sure tokens and ties, read by the cluster
@@ -64,6 +64,7 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int b = g / a.c.Hkv, h = g - b * a.c.Hkv;
   let_next_start();
+  after_previous();
   const int len = min(a.c.len(b), a.w_len), m = min(len, a.budget);
   const float* w = a.weights + b * a.w_bs + h * a.w_hs;
   int* kept = a.kept + static_cast<long long>(g) * a.budget;
@@ -90,71 +91,39 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   const auto weight = [&](int i) { return STAGED ? sw[i - s0] : w[i]; };
   uint32_t T = 0;                                     // the want-th largest key
   int left = want;                                    // ... of whose ties this many are taken
-  for (int i = tid; i < 3 * BINS; i += NT) (&hist[0][0])[i] = 0;
+  for (int i = tid; i < PASSES * BINS; i += NT) (&hist[0][0])[i] = 0;
   __syncthreads();
   if (want > 0) {
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      const int sh = p == 0 ? 21 : p == 1 ? 10 : 0, nbits = p == 2 ? 10 : 11, bins = 1 << nbits;
-      for (int i = max(s0, lo) + tid; i < min(s1, hi); i += NT) {
-        const uint32_t k = key_of(weight(i));
-        if (p == 0 || (k >> (sh + nbits)) == (T >> (sh + nbits))) atomicAdd(&hist[p][(k >> sh) & (bins - 1)], 1);
+    for (int p = 0; p < PASSES; ++p) {
+      const int sh = 32 - DIGIT * (p + 1), a0 = max(s0, lo), a1 = min(s1, hi);
+      for (int i = a0 + tid; i < a1; i += 4 * NT) {
+        uint32_t k[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = i + e * NT < a1 ? key_of(weight(i + e * NT)) : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e * NT < a1 && (p == 0 || (k[e] ^ T) >> ((sh + DIGIT) & 31) == 0)) atomicAdd(&hist[p][(k[e] >> sh) & (BINS - 1)], 1);
       }
       sync();
-      // Counts from the top bin down.  A cluster adds its histograms slice by slice: CTA r the slice of bins/C bins that is
-      // r-th from the top, in place (only r reads or writes it from then on, until the others look the slice of the answer up).
-      int first = 0, width = bins, owner = rank, before = 0;   // slice: bins [top - first - width + 1, top - first]
-      const int top = bins - 1;
-      if (CL) {
-        width = bins / C;
-        first = rank * width;
-        int sum = 0;
-        for (int q = tid; q < width; q += NT) {
-          int n[8], t = 0;
+      // counts from the top bin down, a thread per bin; every CTA of a cluster adds all histograms up for itself
+      const int bin = BINS - 1 - tid;
+      int n = 0;
+      if (tid < BINS) {
+        if (CL) {
+          int x[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) n[r] = r < C ? cl.map_shared_rank(&hist[p][0], r)[top - first - q] : 0;
+          for (int r = 0; r < 8; ++r) x[r] = r < C ? cl.map_shared_rank(&hist[p][0], r)[bin] : 0;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) t += n[r];
-          hist[p][top - first - q] = t;
-          sum += t;
+          for (int r = 0; r < 8; ++r) n += x[r];
+        } else {
+          n = hist[p][bin];
         }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane == 0) red[wid] = sum;
-        __syncthreads();
-        if (tid == 0) {
-          int t = 0;
-          for (int i = 0; i < NWARP; ++i) t += red[i];
-          s_slice[p] = t;
-        }
-        sync();
-        owner = 0;
-        int n[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) n[r] = r < C ? *cl.map_shared_rank(&s_slice[p], r) : 0;
-#pragma unroll
-        for (int r = 0; r < 7; ++r)
-          if (owner == r && before + n[r] < left) before += n[r], owner = r + 1;
-        first = owner * width;
       }
-      // the bin of the slice in which the count reaches `left`
-      const int per = BINS / NT;
-      const int* hs = CL ? cl.map_shared_rank(&hist[p][0], owner) : &hist[p][0];
-      int n[per], mine = 0;
-#pragma unroll
-      for (int e = 0; e < per; ++e) {
-        const int q = tid * per + e;
-        n[e] = q < width ? hs[top - first - q] : 0;
-        mine += n[e];
-      }
-      int cum = before + block_scan(mine, red);
-#pragma unroll
-      for (int e = 0; e < per; ++e) {
-        if (cum < left && left <= cum + n[e]) {       // one bin of one thread
-          s_digit = static_cast<uint32_t>(top - first - (tid * per + e));
-          s_left = left - cum;
-        }
-        cum += n[e];
+      const int cum = block_scan(n, red);
+      if (cum < left && left <= cum + n) {              // the one bin in which the count reaches `left`
+        s_digit = static_cast<uint32_t>(bin);
+        s_left = left - cum;
       }
       __syncthreads();
       T |= s_digit << sh;
@@ -164,18 +133,26 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   }
   // a warp's positions are consecutive: sure tokens (forced, or above T) and ties are counted, then written, 32 at a time
   const int wseg = ((seg + NWARP - 1) / NWARP + 31) & ~31, i0 = min(s0 + wid * wseg, s1), i1 = min(i0 + wseg, s1);
-  const auto kind = [&](int i, bool& tie) {           // sure to be kept; or a tie
-    if (i < lo || i >= hi) return i < i1;
-    const uint32_t k = i < i1 ? key_of(weight(i)) : 0u;
-    tie = i < i1 && want > 0 && k == T;
-    return i < i1 && want > 0 && k > T;
+  // four groups of 32 at a time: bit l of sure / tie = position i + 32 e + l is kept for certain / is a tie
+  constexpr int GR = 4;
+  const auto groups = [&](int i, unsigned (&sure)[GR], unsigned (&tie)[GR]) {
+    uint32_t k[GR];
+#pragma unroll
+    for (int e = 0; e < GR; ++e) k[e] = i + 32 * e + lane < i1 ? key_of(weight(i + 32 * e + lane)) : 0u;
+#pragma unroll
+    for (int e = 0; e < GR; ++e) {
+      const int j = i + 32 * e + lane;
+      const bool forced = j < lo || j >= hi;
+      sure[e] = __ballot_sync(~0u, j < i1 && (forced || (want > 0 && k[e] > T)));
+      tie[e] = __ballot_sync(~0u, j < i1 && !forced && want > 0 && k[e] == T);
+    }
   };
   int sure = 0, ties = 0;
-  for (int i = i0; i < i1; i += 32) {
-    bool tie = false;
-    const bool s = kind(i + lane, tie);
-    sure += __popc(__ballot_sync(~0u, s));
-    ties += __popc(__ballot_sync(~0u, tie));
+  for (int i = i0; i < i1; i += 32 * GR) {
+    unsigned ms[GR], mt[GR];
+    groups(i, ms, mt);
+#pragma unroll
+    for (int e = 0; e < GR; ++e) sure += __popc(ms[e]), ties += __popc(mt[e]);
   }
   if (lane == 0) s_sure[wid] = sure, s_ties[wid] = ties;
   __syncthreads();
@@ -191,29 +168,38 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   if (CL) {
     if (tid == 0) s_count[0] = sure, s_count[1] = ties;
     sync();
-    for (int r = 0; r < rank; ++r) {
-      const int* c = cl.map_shared_rank(&s_count[0], r);
-      const int t = c[1];
-      cta_pos += c[0] + min(max(left - cta_tie, 0), t);
-      cta_tie += t;
+    int x[8], t[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int* c = cl.map_shared_rank(&s_count[0], r < rank ? r : rank);
+      x[r] = r < rank ? c[0] : 0;
+      t[r] = r < rank ? c[1] : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      cta_pos += x[r] + min(max(left - cta_tie, 0), t[r]);
+      cta_tie += t[r];
     }
   }
   int tie_at = cta_tie + tie0;
   pos += cta_pos + min(tie_at, left) - min(cta_tie, left);
   const unsigned below = (1u << lane) - 1;
-  for (int i = i0; i < i1; i += 32) {
-    bool tie = false;
-    bool take = kind(i + lane, tie);
-    const unsigned mt = __ballot_sync(~0u, tie);
-    if (tie) take = tie_at + __popc(mt & below) < left;
-    const unsigned mk = __ballot_sync(~0u, take);
-    if (take) {
-      const int at = pos + __popc(mk & below);
-      kept[at] = i + lane;
-      nw[at] = weight(i + lane);
+  for (int i = i0; i < i1; i += 32 * GR) {
+    unsigned ms[GR], mt[GR];
+    groups(i, ms, mt);
+#pragma unroll
+    for (int e = 0; e < GR; ++e) {
+      // of the ties the first left - tie_at are taken
+      const bool tk = (mt[e] >> lane & 1) && tie_at + __popc(mt[e] & below) < left;
+      const unsigned mk = ms[e] | __ballot_sync(~0u, tk);
+      if (mk >> lane & 1) {
+        const int at = pos + __popc(mk & below), j = i + 32 * e + lane;
+        kept[at] = j;
+        nw[at] = weight(j);
+      }
+      tie_at += __popc(mt[e]);
+      pos += __popc(mk);
     }
-    tie_at += __popc(mt);
-    pos += __popc(mk);
   }
   if (CL) sync();                                     // the others have read this CTA's counts
 }
@@ -224,7 +210,6 @@ template <int D> __global__ void __launch_bounds__(CT) k_copy(EvictArgs a, int c
   constexpr int PPR = D / 8, PPT = 2 * PPR;           // pieces per row, per token (key row, then value row)
   __shared__ long long src[TOK], dst[TOK];            // element offsets of the key rows, or -1 | -2
   const int g = blockIdx.x / chunks, b = g / a.c.Hkv, h = g - b * a.c.Hkv, r0 = (blockIdx.x - g * chunks) * TOK;
-  let_next_start();
   after_previous();
   const int m = a.new_lens[b];
   if (r0 >= m) return;
@@ -264,7 +249,6 @@ template <int D> __global__ void __launch_bounds__(NT) k_move(EvictArgs a, int C
   constexpr int PPR = D / 8, PPT = 2 * PPR, IT = 8, R = IT * NT / PPT;   // tokens per CTA and step
   cg::cluster_group cl = cg::this_cluster();
   const int g = blockIdx.x / C, rank = blockIdx.x - g * C, b = g / a.c.Hkv, h = g - b * a.c.Hkv;
-  let_next_start();
   after_previous();
   const int len = min(a.c.len(b), a.w_len), m = a.new_lens[b];
   if (len <= a.budget) return;                        // (the whole cluster)
@@ -337,21 +321,21 @@ cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
     static std::atomic<bool> done[2][MAX_DEVICES];
     int dev = 0, sms = 0;
     if ((e = device_sms(dev, sms)) || (e = allow_smem(k, MAX_KEYS * 4, dev, done[c > 1]))) return e;
-    e = launch(k, static_cast<unsigned>(groups * c), NT, static_cast<size_t>(seg) * 4, c, false, st, a, c);
+    e = launch(k, static_cast<unsigned>(groups * c), NT, static_cast<size_t>(seg) * 4, c, st, a, c);
   } else {                                            // (the largest cluster)
-    e = launch(k_select<false, true>, static_cast<unsigned>(groups * c), NT, 0, c, false, st, a, c);
+    e = launch(k_select<false, true>, static_cast<unsigned>(groups * c), NT, 0, c, st, a, c);
   }
   if (e != cudaSuccess) return e;
   if (!a.dst_bt) {
     const int cm = cluster_of(groups, a.budget);
-    return a.D == 128 ? launch(k_move<128>, static_cast<unsigned>(groups * cm), NT, 0, cm, true, st, a, cm)
-                      : launch(k_move<64>, static_cast<unsigned>(groups * cm), NT, 0, cm, true, st, a, cm);
+    return a.D == 128 ? launch(k_move<128>, static_cast<unsigned>(groups * cm), NT, 0, cm, st, a, cm)
+                      : launch(k_move<64>, static_cast<unsigned>(groups * cm), NT, 0, cm, st, a, cm);
   }
   const long long longest = width < a.budget ? width : a.budget, chunks = (longest + TOK - 1) / TOK;
   if (chunks == 0) return cudaSuccess;
   if (chunks * groups > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  return a.D == 128 ? launch(k_copy<128>, static_cast<unsigned>(groups * chunks), CT, 0, 0, true, st, a, static_cast<int>(chunks))
-                    : launch(k_copy<64>, static_cast<unsigned>(groups * chunks), CT, 0, 0, true, st, a, static_cast<int>(chunks));
+  return a.D == 128 ? launch(k_copy<128>, static_cast<unsigned>(groups * chunks), CT, 0, 0, st, a, static_cast<int>(chunks))
+                    : launch(k_copy<64>, static_cast<unsigned>(groups * chunks), CT, 0, 0, st, a, static_cast<int>(chunks));
 }
 
 }  // namespace k16

@@ -1,10 +1,10 @@
 // Launches of the 16-bit cache's kernels.
 //
-// All but the eviction's selection are launched programmatically: CTAs may become resident while the stream's previous kernel
-// still runs, and each waits (after_previous) for that kernel's end before it touches global memory.  No thread block returns
-// before that, so a kernel never ends before the one in front of it, and a stream's order holds.  It hides 2 to 4 us of a
-// launch (decode of 32 x 1028 visible tokens: 38.6 -> 34.3 us with the join's loads batched); the clusters of the selection
-// took 3 to 5 us longer that way.
+// Every kernel is launched programmatically: its CTAs may become resident while the stream's previous kernel still runs, and
+// each waits (after_previous) for that kernel's end before it touches global memory.  No thread block returns before that, so a
+// kernel never ends before the one in front of it, and a stream's order holds.  It hides 2 to 4 us of a launch (decode of 32 x
+// 1028 visible tokens: 38.6 -> 34.3 us together with the batched join).  The eviction's copies do not invite the next kernel
+// early (let_next_start): a next selection's clusters that wait beside them cost 5 us.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -37,8 +37,7 @@ template <class K> cudaError_t allow_smem(K kernel, int bytes, int dev, std::ato
 }
 
 template <class... Ts>
-cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, size_t smem, int cluster, bool early, cudaStream_t st,
-                   const Ts&... args) {
+cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, size_t smem, int cluster, cudaStream_t st, const Ts&... args) {
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(grid);
@@ -46,15 +45,14 @@ cudaError_t launch(void (*k)(Ts...), unsigned grid, unsigned threads, size_t sme
   c.dynamicSmemBytes = smem;
   c.stream = st;
   c.attrs = at;
-  if (early) {
-    at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.numAttrs = 1;
   if (cluster > 0) {
-    at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[c.numAttrs].val.clusterDim.x = cluster;
-    at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
-    ++c.numAttrs;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.numAttrs = 2;
   }
   return cudaLaunchKernelEx(&c, k, args...);
 }

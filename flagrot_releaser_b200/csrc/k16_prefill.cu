@@ -675,7 +675,7 @@ cudaError_t launch_p(const PrefillArgs& a, const CUtensorMap& qm, const CUtensor
   const auto k = k_prefill<DT, D>;
   static std::atomic<bool> done[MAX_DEVICES];
   if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, true, st, a, qm, kv, hb, nhg, box, slots);
+  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, st, a, qm, kv, hb, nhg, box, slots);
 }
 
 }  // namespace
