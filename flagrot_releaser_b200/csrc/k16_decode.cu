@@ -17,6 +17,10 @@
 // tiles of 8 q heads: a block goes to one, two or all four warps.  A consumer's MMA has 16 query rows; 8 are q heads and the
 // other 8 carry, in the second product, the rounding errors of the weights: p = hi + lo, both of the cache's type, at no
 // extra cost, so a weight meets the values with an error of 2^-17 instead of 2^-9.
+//
+// Measured (bf16, D 128, G 4, page 16, of the measured copy rate of 6.55 TB/s): 64 rows of up to 4096 tokens 153 us = 0.95; one
+// row of 131072 94 us = 0.87; 32 rows x 1028 visible of 16384 29 us = 0.72; one row of 77 tokens 5 us on the device.  What is
+// left: 4 to 6 us from the launch to a CTA's first block, 2 us for a join's fence and ticket, and the CTAs' uneven ends.
 #include "k16_kernels.h"
 #include "k16_launch.cuh"
 #include "k16_tma.cuh"
