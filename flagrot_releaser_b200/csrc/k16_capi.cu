@@ -68,11 +68,13 @@ int k16_write(const void* kv, long long kv_ts, long long kv_hs, const long long*
 }
 
 long long k16_ws_bytes(int rows, int Hkv, int G, int D, long long max_len, int weights, long long new_tokens) {
+  if (rows < 0 || Hkv < 1 || G < 1 || G > 4096 || (D != 64 && D != 128) || max_len < 0 || new_tokens < 0) return -3;
   const long long a = attn_ws_bytes(rows, Hkv, G, D, max_len, weights);
   const long long p = new_tokens > 0 ? prefill_ws_bytes(rows, Hkv, G, D, new_tokens) : 0;
   return a > p ? a : p;
 }
 long long k16_ws_tickets(int rows, int Hkv, int G, long long new_tokens) {
+  if (rows < 0 || Hkv < 1 || G < 1 || G > 4096 || new_tokens < 0) return -3;
   const long long a = static_cast<long long>(rows) * Hkv * G;
   const long long p = new_tokens > 0 ? prefill_tickets(rows, Hkv, G, new_tokens) : 0;
   return a > p ? a : p;
@@ -87,7 +89,9 @@ int k16_attn(int dtype, const void* q, long long q_bs, const void* pool, long lo
   if (G < 1 || G > 4096 || sinks < 0 || static_cast<long long>(B) * Hkv * G > (1 << 28)) return -3;
   if (B == 0) return 0;
   if (!q || !out || !al16(q) || !al16(out) || q_bs % 8 || o_bs % 8) return -3;
-  if (weights && (w_bs < 0 || w_hs < 0)) return -3;
+  // rows that are written must not be one another's
+  if (B > 1 && o_bs < static_cast<long long>(Hkv) * G * D) return -3;
+  if (weights && (w_bs < 0 || w_hs < 0 || (B > 1 && w_bs == 0) || (Hkv > 1 && w_hs == 0))) return -3;
   if (!tickets || !ws || !al16(ws) || n_tickets < k16_ws_tickets(B, Hkv, G, 0) ||
       ws_bytes < attn_ws_bytes(B, Hkv, G, D, static_cast<long long>(bt_width) * page, weights != nullptr))
     return -4;
@@ -120,6 +124,7 @@ int k16_prefill(int dtype, const void* q, long long q_ts, int T, const int* cu_q
   if (G < 1 || G > 4096 || sinks < 0 || T < 0 || static_cast<long long>(T) * Hkv * G > INT_MAX / 2) return -3;
   if (B == 0 || T == 0) return 0;
   if (!q || !out || !cu_q || !al16(q) || !al16(out) || q_ts % 8 || o_ts % 8) return -3;
+  if (T > 1 && (q_ts < 1 || o_ts < static_cast<long long>(Hkv) * G * D)) return -3;
   if (!tickets || !ws || !al16(ws) || n_tickets < prefill_tickets(B, Hkv, G, T) || ws_bytes < prefill_ws_bytes(B, Hkv, G, D, T))
     return -4;
   PrefillArgs a;
@@ -149,7 +154,7 @@ int k16_evict(const void* pool, long long num_pages, const int* block_table, lon
   if (budget < 1 || budget > (1 << 30) || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > budget) return -3;
   if (w_len < 0 || w_bs < 0 || w_hs < 0 || nw_len < budget || static_cast<long long>(B) * Hkv > 65535 * 16ll) return -3;
   if (B == 0) return 0;
-  if (!weights || !kept || !new_lens || !new_weights) return -3;
+  if ((w_len > 0 && !weights) || !kept || !new_lens || !new_weights) return -3;
   EvictArgs a;
   a.dst = static_cast<uint16_t*>(dst_pool);
   a.dst_pages = dst_pages;

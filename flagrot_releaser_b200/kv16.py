@@ -16,6 +16,7 @@ Pool: torch tensor [num_pages, Hkv, 2, page, D], contiguous, bf16 or fp16 (index
 
 The library must exist (built by flagrot_releaser_b200/_build.py): there is no fallback.  FLAGROT_KV16_LIB overrides its
 location.  All launches go to torch's current CUDA stream and are asynchronous; the tensors have to be on the current device.
+Capture a call in a CUDA graph after it has run once.
 """
 from __future__ import annotations
 
@@ -97,6 +98,7 @@ class Workspace:
 
     def __init__(self, rows, Hkv, G, D, max_len, device, weights=False, new_tokens=0):
         L = lib()
+        assert rows >= 0 and Hkv > 0 and G > 0 and D in HEAD_DIMS and max_len >= 0 and new_tokens >= 0
         self.nbytes = int(L.k16_ws_bytes(rows, Hkv, G, D, max_len, int(weights), new_tokens))
         self.ntickets = int(L.k16_ws_tickets(rows, Hkv, G, new_tokens))
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)

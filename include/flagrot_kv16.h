@@ -10,7 +10,8 @@
  * What lies in a page behind a sequence's length is never used, whatever it holds (NaN included).
  *
  * Every entry takes raw DEVICE pointers, element strides and the caller's cudaStream_t (as void*); launches are
- * asynchronous, allocate nothing and may be captured in CUDA graphs.  The stream must belong to the current device.
+ * asynchronous, allocate nothing and may be captured in CUDA graphs (after a first call on the device outside a capture, which
+ * loads the kernels).  The stream must belong to the current device.
  * Return: 0 ok, -1 launch error (text in k16_last_error), -2 unsupported dtype / head dim / page, -3 bad argument (null or
  * misaligned pointer, negative or too large size), -4 workspace too small.  Nothing is launched when the code is not 0. */
 #ifndef FLAGROT_KV16_H
@@ -34,9 +35,10 @@ int k16_chunk_bytes(int page, int D);
 int k16_write(const void* kv, long long kv_ts, long long kv_hs, const long long* slots, int T, int Hkv, int D, int page,
               long long num_pages, void* pool, void* stream);
 
-/* Workspace of k16_attn / k16_prefill: bytes for up to `rows` sequences of up to max_len cached tokens; weights != 0 when
+/* Workspace of k16_attn / k16_prefill (-3: bad argument): bytes for up to `rows` sequences of up to max_len cached tokens; weights != 0 when
  * k16_attn is called with weights; new_tokens: the largest T of k16_prefill (0: k16_attn only).  tickets: int32, zero before
- * the first call, left zero by every call.  Calls that may overlap on the device need workspaces of their own. */
+ * the first call, left zero by every call (a workspace whose call's wait gave up is void).  Calls that may overlap on the device
+ * need workspaces of their own. */
 long long k16_ws_bytes(int rows, int Hkv, int G, int D, long long max_len, int weights, long long new_tokens);
 long long k16_ws_tickets(int rows, int Hkv, int G, long long new_tokens);
 
@@ -44,7 +46,7 @@ long long k16_ws_tickets(int rows, int Hkv, int G, long long new_tokens);
  * and (window <= 0 or j >= len - window or j < sinks); qscale = softmax scale * log2(e); out [B, G*Hkv*D] (row stride
  * o_bs); q and out rows 16-byte aligned.  A row that sees no key is written as zeros.
  * weights fp32 (or null): weights[b * w_bs + h * w_hs + j] += the softmax weights of visible key j summed over the G heads of
- * kv head h; other entries are left as they are.  Each row needs at least bt_width * page entries. */
+ * kv head h; other entries are left as they are.  Each row needs at least bt_width * page entries, rows of its own. */
 int k16_attn(int dtype, const void* q, long long q_bs, const void* pool, long long num_pages, const int* block_table,
              long long bt_stride, int bt_width, const int* seq_lens, int B, int Hkv, int G, int D, int page, float qscale,
              int window, int sinks, float* weights, long long w_bs, long long w_hs, int* tickets, long long n_tickets, void* ws,

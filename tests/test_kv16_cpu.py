@@ -37,7 +37,8 @@ BAD_CACHE = [(dict(D=96), -2), (dict(page=24), -2), (dict(page=256), -2), (dict(
 
 @pytest.mark.parametrize("kw,rc", BAD_CACHE + [
     (dict(dtype=2), -2), (dict(G=0), -3), (dict(sinks=-1), -3), (dict(q=None), -3), (dict(q=A + 2), -3), (dict(q_bs=1020), -3),
-    (dict(out=None), -3), (dict(out=A + 8), -3), (dict(o_bs=4), -3), (dict(weights=A, w_bs=-1), -3), (dict(tickets=None), -4),
+    (dict(out=None), -3), (dict(out=A + 8), -3), (dict(o_bs=4), -3), (dict(weights=A, w_bs=-1), -3), (dict(weights=A, w_bs=0, w_hs=128), -3), (dict(weights=A, w_bs=256, w_hs=0), -3),
+    (dict(o_bs=1016), -3), (dict(o_bs=0), -3), (dict(tickets=None), -4),
     (dict(nt=1), -4), (dict(ws=None), -4), (dict(wsb=16), -4), (dict(B=1 << 28, Hkv=64), -3)])
 def test_attn_refusals(kw, rc):
     assert _attn(**kw) == rc
@@ -59,7 +60,7 @@ def _prefill(**kw):
 
 @pytest.mark.parametrize("kw,rc", BAD_CACHE + [
     (dict(dtype=-1), -2), (dict(G=0), -3), (dict(sinks=-1), -3), (dict(T=-1), -3), (dict(q=None), -3), (dict(q=A + 4), -3),
-    (dict(q_ts=1028), -3), (dict(cu=None), -3), (dict(out=None), -3), (dict(o_ts=12), -3), (dict(T=1 << 30), -3), (dict(ws=None), -4)])
+    (dict(q_ts=1028), -3), (dict(q_ts=0), -3), (dict(o_ts=512), -3), (dict(cu=None), -3), (dict(out=None), -3), (dict(o_ts=12), -3), (dict(T=1 << 30), -3), (dict(ws=None), -4)])
 def test_prefill_refusals(kw, rc):
     assert _prefill(**kw) == rc
 
@@ -101,6 +102,17 @@ def test_workspace_sizes_grow_with_the_call():
     assert L.k16_ws_bytes(64, 8, 4, 128, 4096, 1, 0) >= n + 64 * 8 * 4 * 4096 * 4
     assert L.k16_ws_bytes(64, 8, 4, 128, 4096, 0, 65536) >= n
     assert L.k16_ws_tickets(64, 8, 4, 0) >= 64 * 8
+    for bad in ((-1, 8, 4, 128, 64, 0, 0), (1, 0, 4, 128, 64, 0, 0), (1, 8, 0, 128, 64, 0, 5), (1, 8, 4, 100, 64, 0, 0), (1, 8, 4, 128, -1, 0, 0),
+                (1, 8, 4, 128, 64, 0, -1)):
+        assert L.k16_ws_bytes(*bad) == -3
+    assert L.k16_ws_tickets(1, 8, 0, 5) == -3 and L.k16_ws_tickets(-1, 8, 4, 0) == -3
+    # a workspace serves every smaller call: the sizes grow in each argument
+    base = (3, 2, 3, 64, 100, 0, 50)
+    for i, v in ((0, 7), (1, 4), (2, 12), (2, 40), (2, 130), (3, 128), (4, 5000), (5, 1), (6, 9000)):
+        more = list(base)
+        more[i] = v
+        assert L.k16_ws_bytes(*more) >= L.k16_ws_bytes(*base)
+        assert L.k16_ws_tickets(more[0], more[1], more[2], more[6]) >= L.k16_ws_tickets(base[0], base[1], base[2], base[6])
     assert kv16.chunk_bytes(16, 128) == L.k16_chunk_bytes(16, 128) == 16 * 128 * 2 * 2
 
 

@@ -465,6 +465,46 @@ def test_evict_ties_infinities_nan_and_signs(K):
             check_evict(K, [n] * 4, 2, 64, 16, BF, budget, 0, budget // 3, 23, in_place, weights=w)
 
 
+def test_evict_to_other_pages_of_the_same_pool(K):
+    g = gen(25)
+    lens, Hkv, budget = [300, 90, 40], 2, 64
+    pool, bt, ln = R.make_cache(lens, Hkv, 64, 16, BF, g, spare=12, poison=False)
+    w = torch.rand(3, Hkv, bt.shape[1] * 16, generator=g).to(DEV)
+    used = set(bt[0, :19].tolist()) | set(bt[1, :6].tolist()) | set(bt[2, :3].tolist())
+    free = torch.tensor([p for p in range(pool.shape[0]) if p not in used][:12], dtype=torch.int32, device=DEV).view(3, 4)
+    kept, nl = torch.empty(3, Hkv, budget, dtype=torch.int32, device=DEV), torch.empty(3, dtype=torch.int32, device=DEV)
+    nw, before = torch.empty(3, Hkv, budget, device=DEV), pool.clone()
+    K.evict(pool, bt, ln, w, budget, 4, 16, kept, nl, nw, dst_table=free)
+    exp = before.clone()
+    for b, n in enumerate(lens):
+        ref = R.evict_ref(w[b], n, budget, 4, 16)
+        for h in range(Hkv):
+            idx, at = torch.tensor(ref[h], device=DEV), torch.arange(len(ref[h]), device=DEV)
+            assert kept[b, h, :len(ref[h])].tolist() == ref[h]
+            exp[free[b, at // 16].long(), h, :, at % 16] = before[bt[b, idx // 16].long(), h, :, idx % 16]
+    assert torch.equal(pool, exp)
+
+
+def test_empty_tables_and_batches(K):
+    pool = torch.zeros(2, 1, 2, 16, 64, dtype=BF, device=DEV)
+    ws = K.Workspace(2, 1, 4, 64, 0, DEV, weights=True, new_tokens=4)
+    bt, ln = torch.zeros(2, 0, dtype=torch.int32, device=DEV), torch.tensor([5, 0], dtype=torch.int32, device=DEV)
+    q, out, w = torch.ones(2, 4, 64, dtype=BF, device=DEV), torch.ones(2, 256, dtype=BF, device=DEV), torch.zeros(2, 1, 0, device=DEV)
+    K.attn(q, pool, bt, ln, out, ws, 0.1, weights=w)
+    assert bool((out == 0).all())
+    out.fill_(1)
+    K.prefill(q, torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), pool, bt, ln, out, 0.1, ws=ws)
+    assert bool((out == 0).all())
+    kept, nl, nw = torch.zeros(2, 1, 3, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV), torch.ones(2, 1, 3, device=DEV)
+    K.evict(pool, bt, ln, w, 3, 1, 1, kept, nl, nw)
+    assert bool((kept == -1).all()) and bool((nl == 0).all()) and bool((nw == 0).all())
+    z = torch.zeros(0, dtype=torch.int32, device=DEV)
+    K.attn(q[:0], pool, bt[:0], z, out[:0], ws, 0.1)
+    K.write(torch.zeros(0, 2, 64, dtype=BF, device=DEV), torch.zeros(0, dtype=torch.int64, device=DEV), pool)
+    K.evict(pool, bt[:0], z, w[:0], 3, 1, 1, kept[:0], nl[:0], nw[:0])
+    assert bool((pool == 0).all())
+
+
 def test_evict_weights_shorter_than_the_table(K):
     """a row is taken as long as its weights at most"""
     w = torch.rand(2, 2, 100, generator=gen(24))
