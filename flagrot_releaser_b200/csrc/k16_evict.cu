@@ -11,7 +11,7 @@
 //
 // Measured (D 128): 32 rows of up to 4096 tokens x 8 heads to 2048: 101 us, of which the copy 82 (the measured copy rate); one row of
 // 60000 x 8 heads to 7500: 34 us, of which the copy 10 and the selection, eight clusters of eight CTAs that meet six times, most
-// of the rest.  In place: 128 and 54 us (a step's reads and the writes of the step before it overlap, the next one's do not).
+// of the rest.  In place: 120 and 54 us (a step's reads and the writes of the step before it overlap, the next one's do not).
 #include <cooperative_groups.h>
 
 #include "k16_kernels.h"
@@ -315,7 +315,9 @@ template <int D, bool CL> __global__ void __launch_bounds__(MT, 2) k_move(EvictA
   }
 }
 
-// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each, and to hold the keys in shared memory
+// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each, and to hold the weights in shared memory.
+// 32 x 4096 x 8 heads: 101 us with one CTA, 131 with four, 174 with eight; 1 x 60000 x 8 heads: 45 with four, 34 with eight, 51 with
+// eight that read the weights again in every pass.
 int cluster_of(long long groups, long long positions) {
   int c = 1;
   while (c < 8 && ((groups * c < 148 && positions / c > 2048) || positions / c > MAX_KEYS)) c *= 2;
@@ -342,8 +344,10 @@ cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
   }
   if (e != cudaSuccess) return e;
   if (!a.dst_bt) {
-    int cm = 1;                                       // two CTAs per SM, a few steps each
-    while (cm < 8 && groups * cm < 2 * 148 && a.budget / cm > 256) cm *= 2;
+    // a CTA per (row, kv head) where they fill the SMs, else a cluster (256 of them: 119 us with one CTA, 127 with two, 138 with
+    // eight; 8 of them: 211, 138 and 53 us)
+    int cm = 1;
+    while (cm < 8 && groups * cm < 148 && a.budget / cm > 256) cm *= 2;
     const auto k = a.D == 128 ? (cm > 1 ? k_move<128, true> : k_move<128, false>) : (cm > 1 ? k_move<64, true> : k_move<64, false>);
     return launch(k, static_cast<unsigned>(groups * cm), MT, 0, cm, st, a, cm);
   }

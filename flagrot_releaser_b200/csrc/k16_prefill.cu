@@ -12,7 +12,8 @@
 // keys through one ring).  S and P go in halves of 64 keys: a half's scores are computed while the other half's weights
 // are, and a half that no query of the tile sees is left out.  The softmax reference is lazy: it moves when a row's
 // maximum has grown by more than 2^8, and only then is O rescaled.
-// Full waves of pairs run whole; the pairs of the last, partly filled wave are cut along their keys and joined.
+// Full waves of pairs run whole; the pairs of the last, partly filled wave are cut along their keys and joined where that is
+// shorter (4 x 512 over 32768: 1117 us with, 1163 without; the window case, whose pairs have 10 blocks: 418 with, 406 without).
 //
 // V is taken as it lies (keys by dims): the second product's B operand is MN-major, K = keys.
 // P is rounded to the cache's type (2^-9 relative in bf16, 2^-12 in fp16: one rounding, like the output's own, which makes
@@ -20,7 +21,7 @@
 //
 // Measured (bf16, D 128, G 4, page 16): 4 x 512 new tokens over 32768: 1.09 ms = 1.02 PFLOP/s under the power cap, where the
 // same pipeline without its softmax runs at 1.30 and cuBLAS at 1.40; prompts of 5544 to 7033 tokens through a window of 1024:
-// 0.41 ms = 0.72 PFLOP/s of visible pairs (1216 keys are computed for 1028 visible ones).  A step of 128 keys takes about
+// 0.395 ms = 0.75 PFLOP/s of visible pairs (1216 keys are computed for 1028 visible ones).  A step of 128 keys takes about
 // 3900 cycles, 2500 of them tensor (the N = 64 products of the halves cost 48 cycles instead of 32); the rest is latency of
 // the one softmax warp per tile and scheduler.  Measured and not kept: a polynomial 2^x for part of the weights (the MUFU is
 // half idle), two threads per row (104 registers a thread: spills), whole 128-key S tiles (the same time, windows 8 % slower),
@@ -41,7 +42,7 @@ constexpr int MAX_HEADS = 128;           // q heads per item
 constexpr float LAZY = 8.f;
 constexpr int MAX_SPLIT = 32;            // pieces of a pair's key blocks
 constexpr int SLOTS = 4 * 148;           // workspace slots at most: pieces of split pairs
-constexpr int SPLIT_COST = 4;            // what a piece costs besides its blocks, in blocks
+constexpr int SPLIT_COST = 8;            // what a piece costs besides its blocks, in blocks: its start, its sums' way through the workspace
 
 __device__ int g_status;
 
@@ -161,7 +162,8 @@ FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n
 FR_DEVI float4 f4(const uint32_t* v) {
   return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
 }
-// 16 dims of an output row times inv (zeros when !any); wide: rows are 32-byte aligned, a whole sector per store
+// 16 dims of an output row times inv (zeros when !any); wide: rows are 32-byte aligned, a whole sector per store (the window case:
+// 418 us with, 435 without)
 template <int DT> FR_DEVI void put16(uint16_t* out, float4 x, float4 y, float4 z, float4 t, float inv, bool any, bool wide) {
   uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (any) {
