@@ -13,10 +13,12 @@
 // of the pieces: the result does not depend on which one that is).
 //
 // CTA: four consumer warps and a producer warp that fills a ring of 16 KB stages (one block: 32 keys and their values) with
-// two tensor copies each; two CTAs per SM, so that a CTA's start and joins are covered by the other's stream.  NT = 1 | 2 | 4
-// tiles of 8 q heads: a block goes to one, two or all four warps.  A consumer's MMA has 16 query rows; 8 are q heads and the
-// other 8 carry, in the second product, the rounding errors of the weights: p = hi + lo, both of the cache's type, at no
-// extra cost, so a weight meets the values with an error of 2^-17 instead of 2^-9.
+// two tensor copies each; two CTAs per SM, so that a CTA's start and joins are covered by the other's stream.  A block goes to
+// NT warps, one per tile of TR q heads: one tile of 8 for G up to 8, two of 8 up to 16, two of 16 above.  A weight meets the
+// values as p = hi + lo, both of the cache's type, with an error of 2^-17 instead of 2^-9: in a tile of 8 the other 8 rows of
+// the second MMA carry lo, at no extra cost; in a tile of 16 lo is a product of its own.  Per head that is a quarter fewer MMAs
+// and half the reads of shared memory: G 32 (64 rows of 4096 tokens, 4 kv heads, D 128) 122 us, with four tiles of 8 157;
+// D 64 43 and 53.  G 16 as one tile of 16: 191 us where two of 8 take 177, for a warp then is too long at a block.
 //
 // Measured (bf16, D 128, G 4, page 16, of the measured copy rate of 6.55 TB/s): 64 rows of up to 4096 tokens 153 us = 0.95; one
 // row of 131072 94 us = 0.87; 32 rows x 1028 visible of 16384 29 us = 0.72; one row of 77 tokens 5 us on the device.  What is
@@ -39,14 +41,14 @@ __device__ int g_status;
 // a workspace slot: sums [GT][D], then (reference, denominator) [GT]; a multiple of 16 bytes
 __host__ __device__ __forceinline__ long long slot_floats(int GT, int D) { return (static_cast<long long>(GT) * (D + 2) + 3) & ~3ll; }
 
-template <int D> struct Smem {
+template <int D, int TR> struct Smem {   // TR: q heads of a tile
   // a multiple of NW: a stage always goes to the same warps, whose waits on its barrier then follow its phases one by one
   // (copies of different stages may land in any order, and a parity wait cannot tell a phase from the one two before)
   static constexpr int STAGES = D == 128 ? 4 : 8;
   static constexpr int STAGE = BLK * D * 4;                    // keys, values
-  static constexpr int MERGE = STAGES * STAGE;                 // float [NW][8][D]
-  static constexpr int ML = MERGE + NW * 8 * D * 4;            // float2 [NW][8]
-  static constexpr int BAR = ML + NW * 8 * 8;                  // full[STAGES], empty[STAGES]
+  static constexpr int MERGE = STAGES * STAGE;                 // float [NW][TR][D]
+  static constexpr int ML = MERGE + NW * TR * D * 4;           // float2 [NW][TR]
+  static constexpr int BAR = ML + NW * TR * 8;                 // full[STAGES], empty[STAGES]
   static constexpr int RED = BAR + 2 * STAGES * 8;             // long long [NW + 1]; int [2 (NW + 1)]; abort flag; last-arriver flag
   static constexpr int TOTAL = RED + 96 + 1024;                // slack: the ring starts on a 1024-byte boundary
 };
@@ -228,11 +230,12 @@ FR_DEVI void join(const AttnArgs& a, const float* part, long long quota, long lo
   }
 }
 
-template <int DT, int D, int NT>
+template <int DT, int D, int TR, int NT>
 __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map, int nhg,
                                                        float* part, float* lse, float* scores, long long score_ld) {
-  using S = Smem<D>;
+  using S = Smem<D, TR>;
   constexpr int STAGES = S::STAGES, KS = D / 16, ND = D / 8;                       // k steps of q . k, dim tiles of p . v
+  constexpr int R = TR / 8;                                    // q heads of a thread: rows g and g + 8 of the tile
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
   const uint32_t sm = (raw + 1023) & ~1023u;
@@ -364,20 +367,26 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
     const int h = wk.seg / nhg, hg = wk.seg - h * nhg;
     const int heads = min(a.G - hg * MAX_GT, MAX_GT);          // q heads of the segment
     const int hq0 = h * a.G + hg * MAX_GT;
-    const int hv = heads - tile * 8;                           // ... and of this warp's tile (may be <= 0)
-    uint32_t q[KS][2];
-    {
-      const uint32_t* qr = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + wk.b * a.q_bs + (hq0 + tile * 8 + g) * D);
+    const int hv = heads - tile * TR;                          // ... and of this warp's tile (may be <= 0)
+    uint32_t q[KS][2 * R];
+    // scores of row g (R = 2, and of row g + 8, which need not be one of the segment's)
+    float* const srow = scores && g < hv ? scores + (static_cast<long long>(wk.b) * Hq + hq0 + tile * TR + g) * score_ld + 2 * t : nullptr;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool mine = g + 8 * r < hv;
+      const int hq = hq0 + tile * TR + g + 8 * r;
+      const uint32_t* qr = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + wk.b * a.q_bs + hq * D);
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        q[i][0] = g < hv ? qr[i * 8 + t] : 0u;
-        q[i][1] = g < hv ? qr[i * 8 + 4 + t] : 0u;
+        q[i][r] = mine ? qr[i * 8 + t] : 0u;
+        q[i][R + r] = mine ? qr[i * 8 + 4 + t] : 0u;
       }
     }
-    float o[ND][4], ref = -INFINITY, l = 0.f;
+    float o[ND][4], ref[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) ref[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float* srow = scores && g < hv ? scores + (static_cast<long long>(wk.b) * Hq + hq0 + tile * 8 + g) * score_ld + 2 * t : nullptr;
     const int cnt = wk.k1 - wk.k0;
     for (int i = ((grp - n) % GROUPS + GROUPS) % GROUPS; i < cnt; i += GROUPS) {
       const int st = (n + i) % STAGES;
@@ -392,84 +401,124 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
         for (int c = 0; c < D / 32; ++c) {                     // 32 dims: pieces 4 c .. 4 c + 3
           uint32_t kf[4];
           ldsm4(kt + (nt >> 1) * a16 + (c >> 1) * ahalf + (nt & 1) * 1024 + (kx ^ ((c & 1) << 6)), kf);
-          mma<DT>(s[nt], q[2 * c][0], 0u, q[2 * c][1], 0u, kf[0], kf[1]);
-          mma<DT>(s[nt], q[2 * c + 1][0], 0u, q[2 * c + 1][1], 0u, kf[2], kf[3]);
+          if constexpr (R == 1) {
+            mma<DT>(s[nt], q[2 * c][0], 0u, q[2 * c][1], 0u, kf[0], kf[1]);
+            mma<DT>(s[nt], q[2 * c + 1][0], 0u, q[2 * c + 1][1], 0u, kf[2], kf[3]);
+          } else {
+            mma<DT>(s[nt], q[2 * c][0], q[2 * c][1], q[2 * c][2], q[2 * c][3], kf[0], kf[1]);
+            mma<DT>(s[nt], q[2 * c + 1][0], q[2 * c + 1][1], q[2 * c + 1][2], q[2 * c + 1][3], kf[2], kf[3]);
+          }
         }
       }
       const bool whole = wk.r.whole(blk);
       uint32_t vm[4] = {~0u, ~0u, ~0u, ~0u};                   // values of hidden keys are zeroed: 0 * NaN is NaN
-      float mx = -INFINITY;
+      float mx[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) mx[r] = -INFINITY;
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
-        s[nt][0] *= a.qscale;
-        s[nt][1] *= a.qscale;
-        if (srow) *reinterpret_cast<float2*>(srow + blk * BLK + nt * 8) = make_float2(s[nt][0], s[nt][1]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          s[nt][2 * r] *= a.qscale;
+          s[nt][2 * r + 1] *= a.qscale;
+          if (srow && (r == 0 || g + 8 < hv))
+            *reinterpret_cast<float2*>(srow + r * 8 * score_ld + blk * BLK + nt * 8) = make_float2(s[nt][2 * r], s[nt][2 * r + 1]);
+        }
         if (!whole) {
           const int j = blk * BLK + nt * 8 + 2 * t;
           const bool a0 = wk.r.visible(j), a1 = wk.r.visible(j + 1);
-          if (!a0) s[nt][0] = -INFINITY;
-          if (!a1) s[nt][1] = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (!a0) s[nt][2 * r] = -INFINITY;
+            if (!a1) s[nt][2 * r + 1] = -INFINITY;
+          }
           vm[nt] = (a0 ? 0xFFFFu : 0u) | (a1 ? 0xFFFF0000u : 0u);
         }
-        mx = fmaxf(mx, fmaxf(s[nt][0], s[nt][1]));
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-      if (__any_sync(~0u, mx > ref + LAZY)) {                  // (the first block: ref = -inf)
-        const float nr = fmaxf(mx, ref), f = ex2(ref - nr);
-        ref = nr;
-        l *= f;
 #pragma unroll
-        for (int x = 0; x < ND; ++x) o[x][0] *= f, o[x][1] *= f, o[x][2] *= f, o[x][3] *= f;
+        for (int r = 0; r < R; ++r) mx[r] = fmaxf(mx[r], fmaxf(s[nt][2 * r], s[nt][2 * r + 1]));
+      }
+      bool moves = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 2));
+        moves |= mx[r] > ref[r] + LAZY;
+      }
+      if (__any_sync(~0u, moves)) {                            // (the first block: ref = -inf)
+        float f[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float nr = fmaxf(mx[r], ref[r]);
+          f[r] = ex2(ref[r] - nr);
+          ref[r] = nr;
+          l[r] *= f[r];
+        }
+#pragma unroll
+        for (int x = 0; x < ND; ++x) o[x][0] *= f[0], o[x][1] *= f[0], o[x][2] *= f[R - 1], o[x][3] *= f[R - 1];
       }
       // fp16 weights are carried times 2^6: below 2^-24 its steps are absolute
-      const float off = DT == 1 ? 6.f - ref : -ref;
-      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const float p0 = ex2(s[nt][0] + off), p1 = ex2(s[nt][1] + off);
-        l += p0 + p1;
-        hi[nt] = Elem<DT>::pack(p0, p1);
-        const float2 r = Elem<DT>::f2(hi[nt]);
-        lo[nt] = Elem<DT>::pack(p0 - r.x, p1 - r.y);
-      }
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t hi[2][R], lo[2][R];
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int r = 0; r < R; ++r) {
+          const float off = DT == 1 ? 6.f - ref[r] : -ref[r];
+#pragma unroll
+          for (int n2 = 0; n2 < 2; ++n2) {
+            const float p0 = ex2(s[2 * ks + n2][2 * r] + off), p1 = ex2(s[2 * ks + n2][2 * r + 1] + off);
+            l[r] += p0 + p1;
+            hi[n2][r] = Elem<DT>::pack(p0, p1);
+            const float2 e = Elem<DT>::f2(hi[n2][r]);
+            lo[n2][r] = Elem<DT>::pack(p0 - e.x, p1 - e.y);
+          }
+        }
 #pragma unroll
         for (int c = 0; c < ND; c += 2) {                      // 16 dims: pieces c, c + 1
           uint32_t vf[4];
           ldsm4t(vt + ks * a16 + (c >> 3) * ahalf + (vx ^ ((c & 7) << 4)), vf);
           if (!whole) vf[0] &= vm[2 * ks], vf[1] &= vm[2 * ks + 1], vf[2] &= vm[2 * ks], vf[3] &= vm[2 * ks + 1];
-          mma<DT>(o[c], hi[2 * ks], lo[2 * ks], hi[2 * ks + 1], lo[2 * ks + 1], vf[0], vf[1]);
-          mma<DT>(o[c + 1], hi[2 * ks], lo[2 * ks], hi[2 * ks + 1], lo[2 * ks + 1], vf[2], vf[3]);
+          if constexpr (R == 1) {
+            mma<DT>(o[c], hi[0][0], lo[0][0], hi[1][0], lo[1][0], vf[0], vf[1]);
+            mma<DT>(o[c + 1], hi[0][0], lo[0][0], hi[1][0], lo[1][0], vf[2], vf[3]);
+          } else {
+            mma<DT>(o[c], hi[0][0], hi[0][1], hi[1][0], hi[1][1], vf[0], vf[1]);
+            mma<DT>(o[c + 1], hi[0][0], hi[0][1], hi[1][0], hi[1][1], vf[2], vf[3]);
+            mma<DT>(o[c], lo[0][0], lo[0][1], lo[1][0], lo[1][1], vf[0], vf[1]);
+            mma<DT>(o[c + 1], lo[0][0], lo[0][1], lo[1][0], lo[1][1], vf[2], vf[3]);
+          }
         }
+      }
       __syncwarp();
       if (lane == 0) tc5::mbar_arrive(empty + 8 * st);
     }
     n += cnt;
     // ---- join the warps of a tile, then the CTAs of a segment
-    l += __shfl_xor_sync(~0u, l, 1);
-    l += __shfl_xor_sync(~0u, l, 2);
-    if (t == 0) ml[w * 8 + g] = make_float2(ref, l);
-    float* mw = mo + (w * 8 + g) * D + 2 * t;
-    if (g < hv)
 #pragma unroll
-      for (int x = 0; x < ND; ++x) *reinterpret_cast<float2*>(mw + x * 8) = make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]);
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(~0u, l[r], 1);
+      l[r] += __shfl_xor_sync(~0u, l[r], 2);
+      if (t == 0) ml[w * TR + 8 * r + g] = make_float2(ref[r], l[r]);
+      float* mw = mo + (w * TR + 8 * r + g) * D + 2 * t;
+      if (g + 8 * r < hv)
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+          *reinterpret_cast<float2*>(mw + x * 8) = R == 1 ? make_float2(o[x][0] + o[x][2], o[x][1] + o[x][3]) : make_float2(o[x][2 * r], o[x][2 * r + 1]);
+    }
     bar_consumers();
     const int c0 = wk.first_cta(), c1 = wk.last_cta();
     float* slot = part + (static_cast<long long>(blockIdx.x) * 2 + (wk.f0 + wk.k0 == blockIdx.x * quota ? 0 : 1)) * slot_floats(GT, D);
     for (int i = tid; i < heads * (D / 2); i += 32 * NW) {
-      const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2)), w0 = (hh >> 3) * GROUPS;
+      const int hh = i / (D / 2), d = 2 * (i - hh * (D / 2)), w0 = hh / TR * GROUPS;
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int x = 0; x < GROUPS; ++x) M = fmaxf(M, ml[(w0 + x) * 8 + (hh & 7)].x);
+      for (int x = 0; x < GROUPS; ++x) M = fmaxf(M, ml[(w0 + x) * TR + hh % TR].x);
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < GROUPS; ++x) {
-        const float2 e = ml[(w0 + x) * 8 + (hh & 7)];
+        const float2 e = ml[(w0 + x) * TR + hh % TR];
         if (e.y == 0.f) continue;                              // this warp had no block of the piece
         const float f = ex2(e.x - M);
-        const float2 y = *reinterpret_cast<const float2*>(mo + ((w0 + x) * 8 + (hh & 7)) * D + d);
+        const float2 y = *reinterpret_cast<const float2*>(mo + ((w0 + x) * TR + hh % TR) * D + d);
         L = fmaf(f, e.y, L);
         v.x = fmaf(f, y.x, v.x);
         v.y = fmaf(f, y.y, v.y);
@@ -537,20 +586,20 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_weights(AttnArgs a,
 
 long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
-template <int DT, int D, int NT>
+template <int DT, int D, int TR, int NT>
 cudaError_t launch_d(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                    cudaStream_t st) {
-  const auto k = k_decode<DT, D, NT>;
+  const auto k = k_decode<DT, D, TR, NT>;
   static std::atomic<bool> done[MAX_DEVICES];
-  if (cudaError_t e = allow_smem(k, Smem<D>::TOTAL, dev, done)) return e;
-  return launch(k, grid, THREADS, Smem<D>::TOTAL, 0, st, a, map, nhg, part, lse, scores, ld);
+  if (cudaError_t e = allow_smem(k, Smem<D, TR>::TOTAL, dev, done)) return e;
+  return launch(k, grid, THREADS, Smem<D, TR>::TOTAL, 0, st, a, map, nhg, part, lse, scores, ld);
 }
 template <int DT, int D>
 cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                       cudaStream_t st) {
-  if (a.G <= 8) return launch_d<DT, D, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
-  if (a.G <= 16) return launch_d<DT, D, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
-  return launch_d<DT, D, 4>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 8) return launch_d<DT, D, 8, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 16) return launch_d<DT, D, 8, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  return launch_d<DT, D, 16, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
 }
 
 }  // namespace
