@@ -224,7 +224,7 @@ def evict(pool, block_table, seq_lens, weights, budget, sinks, recent, kept, new
         return
     nwp, wp = new_weights.data_ptr(), weights.data_ptr()
     assert nwp + new_weights.numel() * 4 <= wp or wp + ((B - 1) * wb + (Hkv - 1) * wh + W) * 4 <= nwp, "new_weights overlaps weights"
-    assert new_lens.data_ptr() != seq_lens.data_ptr(), "new_lens must not be seq_lens"
+    assert abs(new_lens.data_ptr() - seq_lens.data_ptr()) >= 4 * B, "new_lens overlaps seq_lens"
     stream = _stream(pool, block_table, seq_lens, weights, kept, new_lens, new_weights)
     dp = dn = dt = ds = dw = 0
     if dst_table is not None:

@@ -140,3 +140,14 @@ def test_front_end_refuses_before_the_library_is_called():
     for args in ((q, cu[:3], pool, bt, lens, out), (q, cu.long(), pool, bt, lens, out), (q, cu, pool, bt, lens, out.float())):
         with pytest.raises(AssertionError):
             kv16.prefill(*args, 0.1)
+
+
+def test_evict_refuses_results_over_its_inputs():
+    pool, bt = torch.zeros(4, 2, 2, 16, 128, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32)
+    w, kept = torch.zeros(3, 2, 32), torch.zeros(3, 2, 16, dtype=torch.int32)
+    lens = torch.zeros(8, dtype=torch.int32)
+    for a, b in ((0, 0), (0, 2), (2, 0)):
+        with pytest.raises(AssertionError, match="new_lens overlaps seq_lens"):
+            kv16.evict(pool, bt, lens[a:a + 3], w, 16, 0, 0, kept, lens[b:b + 3], torch.zeros(3, 2, 16))
+    with pytest.raises(AssertionError, match="new_weights overlaps weights"):
+        kv16.evict(pool, bt, lens[:3], w, 16, 0, 0, kept, lens[3:6], w.view(-1)[96:].view(3, 2, 16))
