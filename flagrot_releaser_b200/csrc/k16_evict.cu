@@ -24,7 +24,7 @@ namespace {
 
 constexpr int NT = 512, NWARP = NT / 32;
 constexpr int DIGIT = 8, BINS = 1 << DIGIT, PASSES = 32 / DIGIT;
-constexpr int MAX_KEYS = 16384;                       // keys of a CTA's positions that shared memory holds
+constexpr int MAX_KEYS = 32 * NT;                     // keys of a CTA that registers hold
 
 // order-preserving key of a weight: a > b as floats iff key(a) > key(b); -0 equals +0, NaN is below everything
 FR_DEVI uint32_t key_of(float w) {
@@ -32,33 +32,18 @@ FR_DEVI uint32_t key_of(float w) {
   const uint32_t u = __float_as_uint(w + 0.f);        // -0 + 0 = +0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-// exclusive sum over the CTA
-FR_DEVI int block_scan(int v, int* red) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int s = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(~0u, s, d);
-    if (lane >= d) s += y;
-  }
-  __syncthreads();
-  if (lane == 31) red[w] = s;
-  __syncthreads();
-  int before = 0;
-#pragma unroll
-  for (int i = 0; i < NWARP; ++i)
-    if (i < w) before += red[i];
-  return before + s - v;
-}
+FR_DEVI float weight_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }   // (0: a NaN)
+// the n lowest of 32 bits
+FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
-// STAGED: the CTA's weights are read once and kept in shared memory (at most MAX_KEYS); else every pass reads them again.
+// A warp's positions are consecutive; lane l has every 32nd of them from the l-th on, KPT keys in registers.  ONCE: that is all
+// of them, read once; else (more than MAX_KEYS to a CTA) every pass reads them again, KPT at a time.
 // CL: the cluster has more than one CTA.
-template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(EvictArgs a, int C) {
-  extern __shared__ float sw[];
-  __shared__ int hist[PASSES][BINS];
-  __shared__ int red[NWARP], s_sure[NWARP], s_ties[NWARP];
-  __shared__ uint32_t s_digit;
-  __shared__ int s_left;
+template <int KPT, bool ONCE, bool CL> __global__ void __launch_bounds__(NT, KPT <= 16 ? 2 : 1) k_select(EvictArgs a, int C) {
+  static_assert(ONCE || KPT == 32, "a mask of 32 positions to a lane");
+  __shared__ alignas(16) int hist[PASSES][BINS];
+  __shared__ alignas(16) int total[BINS];             // the cluster's histogram of a pass
+  __shared__ int s_sure[NWARP], s_ties[NWARP];
   __shared__ int s_count[2];                          // this CTA's sure tokens and ties, read by the cluster
   cg::cluster_group cl = cg::this_cluster();
   const auto sync = [&]() {
@@ -67,6 +52,7 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   };
   const int g = blockIdx.x / C, rank = blockIdx.x - g * C, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int b = g / a.c.Hkv, h = g - b * a.c.Hkv;
+  for (int i = tid; i < PASSES * BINS; i += NT) (&hist[0][0])[i] = 0;
   let_next_start();
   after_previous();
   const int len = min(a.c.len(b), a.w_len), m = min(len, a.budget);
@@ -74,16 +60,16 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   int* kept = a.kept + static_cast<long long>(g) * a.budget;
   float* nw = a.new_weights + static_cast<long long>(g) * a.nw_len;
   const int seg = (len + C - 1) / C, s0 = min(rank * seg, len), s1 = min(s0 + seg, len);
-  if (STAGED && len > a.budget) {                     // eight loads of a thread in flight
-    for (int i = s0 + tid; i < s1; i += 8 * NT) {
-      float x[8];
+  const int wseg = ((seg + NWARP - 1) / NWARP + 31) & ~31, i0 = min(s0 + wid * wseg, s1), i1 = min(i0 + wseg, s1);
+  uint32_t k[KPT];
+  const auto load = [&](int i) {                      // the keys of positions i + 32 e + lane, all loads in flight
+    float x[KPT];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = i + e * NT < s1 ? w[i + e * NT] : 0.f;
+    for (int e = 0; e < KPT; ++e) x[e] = i + 32 * e + lane < i1 ? w[i + 32 * e + lane] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (i + e * NT < s1) sw[i + e * NT - s0] = x[e];
-    }
-  }
+    for (int e = 0; e < KPT; ++e) k[e] = key_of(x[e]);
+  };
+  if (ONCE && len > a.budget) load(i0);
   if (h == 0 && rank == 0 && tid == 0) a.new_lens[b] = m;
   for (int i = m + rank * NT + tid; i < a.budget; i += C * NT) kept[i] = -1;
   for (int i = m + rank * NT + tid; i < a.nw_len; i += C * NT) nw[i] = 0.f;
@@ -92,72 +78,85 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
     return;
   }
   const int lo = a.sinks, hi = len - a.recent, want = a.budget - a.sinks - a.recent;   // [lo, hi) is chosen from
-  const auto weight = [&](int i) { return STAGED ? sw[i - s0] : w[i]; };
+  // bit e: position i + 32 e + lane is among those before n
+  const auto before = [&](int i, int n) { return low_bits((n - i - lane + 31) >> 5); };
+  const auto chosen_from = [&](int i) { return want > 0 ? before(i, min(hi, i1)) & ~before(i, lo) : 0u; };
   uint32_t T = 0;                                     // the want-th largest key
   int left = want;                                    // ... of whose ties this many are taken
-  for (int i = tid; i < PASSES * BINS; i += NT) (&hist[0][0])[i] = 0;
   __syncthreads();
   if (want > 0) {
-#pragma unroll
+#pragma unroll 1
     for (int p = 0; p < PASSES; ++p) {
-      const int sh = 32 - DIGIT * (p + 1), a0 = max(s0, lo), a1 = min(s1, hi);
-      for (int i = a0 + tid; i < a1; i += 4 * NT) {
-        uint32_t k[4];
+      const int sh = 32 - DIGIT * (p + 1);
+      for (int i = i0; i < i1; i += 32 * KPT) {
+        if (!ONCE) load(i);
+        const uint32_t cand = chosen_from(i), top = p == 0 ? 0u : ~0u << (sh + DIGIT);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = i + e * NT < a1 ? key_of(weight(i + e * NT)) : 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + e * NT < a1 && (p == 0 || (k[e] ^ T) >> ((sh + DIGIT) & 31) == 0)) atomicAdd(&hist[p][(k[e] >> sh) & (BINS - 1)], 1);
-      }
-      sync();
-      // counts from the top bin down, a thread per bin; every CTA of a cluster adds all histograms up for itself
-      const int bin = BINS - 1 - tid;
-      int n = 0;
-      if (tid < BINS) {
-        if (CL) {
-          int x[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) x[r] = r < C ? cl.map_shared_rank(&hist[p][0], r)[bin] : 0;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) n += x[r];
-        } else {
-          n = hist[p][bin];
+        for (int e = 0; e < KPT; ++e) {
+          if (i + 32 * e >= i1) break;
+          if ((cand >> e & 1) && ((k[e] ^ T) & top) == 0) atomicAdd(&hist[p][(k[e] >> sh) & (BINS - 1)], 1);
         }
       }
-      const int cum = block_scan(n, red);
-      if (cum < left && left <= cum + n) {              // the one bin in which the count reaches `left`
-        s_digit = static_cast<uint32_t>(bin);
-        s_left = left - cum;
+      sync();
+      const int* cnt = hist[p];
+      if (CL) {                                       // every CTA of a cluster adds all histograms up for itself
+        if (tid < BINS) {
+          int x[8], n = 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) x[r] = r < C ? cl.map_shared_rank(&hist[p][0], r)[tid] : 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) n += x[r];
+          total[tid] = n;
+        }
+        __syncthreads();
+        cnt = total;
       }
-      __syncthreads();
-      T |= s_digit << sh;
-      left = s_left;
-      __syncthreads();
+      // counts from the top bin down, eight bins a lane, every warp for itself: the one bin in which the count reaches `left`
+      const int4* c4 = reinterpret_cast<const int4*>(cnt + BINS - 8 * (lane + 1));
+      const int4 x = c4[0], y = c4[1];
+      const int c8[8] = {y.w, y.z, y.y, y.x, x.w, x.z, x.y, x.x};
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n += c8[e];
+      int cum = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(~0u, cum, d);
+        if (lane >= d) cum += v;
+      }
+      const int src = __ffs(__ballot_sync(~0u, cum >= left)) - 1;
+      int digit = BINS - 1 - 8 * lane, rest = left - (cum - n);
+#pragma unroll
+      for (int e = 0; e < 7; ++e) {
+        const bool on = digit == BINS - 1 - 8 * lane - e && rest > c8[e];
+        rest -= on ? c8[e] : 0;
+        digit -= on ? 1 : 0;
+      }
+      T |= static_cast<uint32_t>(__shfl_sync(~0u, digit, src)) << sh;
+      left = __shfl_sync(~0u, rest, src);
     }
   }
-  // a warp's positions are consecutive: sure tokens (forced, or above T) and ties are counted, then written, 32 at a time
-  const int wseg = ((seg + NWARP - 1) / NWARP + 31) & ~31, i0 = min(s0 + wid * wseg, s1), i1 = min(i0 + wseg, s1);
-  // four groups of 32 at a time: bit l of sure / tie = position i + 32 e + l is kept for certain / is a tie
-  constexpr int GR = 4;
-  const auto groups = [&](int i, unsigned (&sure)[GR], unsigned (&tie)[GR]) {
-    uint32_t k[GR];
+  // sure tokens (forced, or above T) and ties are counted, then written in order, 32 at a time
+  uint32_t msure = 0, mtie = 0;                       // bit e: position i + 32 e + lane is one
+  const auto mark = [&](int i) {
+    const uint32_t cand = chosen_from(i);
+    msure = before(i, i1) & (~before(i, hi) | before(i, lo));
+    mtie = 0;
 #pragma unroll
-    for (int e = 0; e < GR; ++e) k[e] = i + 32 * e + lane < i1 ? key_of(weight(i + 32 * e + lane)) : 0u;
-#pragma unroll
-    for (int e = 0; e < GR; ++e) {
-      const int j = i + 32 * e + lane;
-      const bool forced = j < lo || j >= hi;
-      sure[e] = __ballot_sync(~0u, j < i1 && (forced || (want > 0 && k[e] > T)));
-      tie[e] = __ballot_sync(~0u, j < i1 && !forced && want > 0 && k[e] == T);
+    for (int e = 0; e < KPT; ++e) {
+      msure |= k[e] > T ? cand & (1u << e) : 0u;
+      mtie |= k[e] == T ? cand & (1u << e) : 0u;
     }
   };
   int sure = 0, ties = 0;
-  for (int i = i0; i < i1; i += 32 * GR) {
-    unsigned ms[GR], mt[GR];
-    groups(i, ms, mt);
-#pragma unroll
-    for (int e = 0; e < GR; ++e) sure += __popc(ms[e]), ties += __popc(mt[e]);
+  for (int i = i0; i < i1; i += 32 * KPT) {
+    if (!ONCE) load(i);
+    mark(i);
+    sure += __popc(msure);
+    ties += __popc(mtie);
   }
+  sure = __reduce_add_sync(~0u, sure);
+  ties = __reduce_add_sync(~0u, ties);
   if (lane == 0) s_sure[wid] = sure, s_ties[wid] = ties;
   __syncthreads();
   int pos = 0, tie0 = 0;                              // this CTA's before this warp
@@ -171,7 +170,7 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
   int cta_tie = 0, cta_pos = 0;                       // ties and kept tokens before this CTA
   if (CL) {
     if (tid == 0) s_count[0] = sure, s_count[1] = ties;
-    sync();
+    cl.sync();
     int x[8], t[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
@@ -184,28 +183,30 @@ template <bool STAGED, bool CL> __global__ void __launch_bounds__(NT) k_select(E
       cta_pos += x[r] + min(max(left - cta_tie, 0), t[r]);
       cta_tie += t[r];
     }
+    cl.barrier_arrive();                              // the last look at the others' memory
   }
   int tie_at = cta_tie + tie0;
   pos += cta_pos + min(tie_at, left) - min(cta_tie, left);
   const unsigned below = (1u << lane) - 1;
-  for (int i = i0; i < i1; i += 32 * GR) {
-    unsigned ms[GR], mt[GR];
-    groups(i, ms, mt);
+  for (int i = i0; i < i1; i += 32 * KPT) {
+    if (!ONCE) load(i), mark(i);
 #pragma unroll
-    for (int e = 0; e < GR; ++e) {
+    for (int e = 0; e < KPT; ++e) {
+      if (i + 32 * e >= i1) break;
       // of the ties the first left - tie_at are taken
-      const bool tk = (mt[e] >> lane & 1) && tie_at + __popc(mt[e] & below) < left;
-      const unsigned mk = ms[e] | __ballot_sync(~0u, tk);
-      if (mk >> lane & 1) {
-        const int at = pos + __popc(mk & below), j = i + 32 * e + lane;
-        kept[at] = j;
-        nw[at] = weight(j);
+      const unsigned mt = __ballot_sync(~0u, mtie >> e & 1);
+      const bool mine = (msure >> e & 1) || ((mtie >> e & 1) && tie_at + __popc(mt & below) < left);
+      const unsigned mk = __ballot_sync(~0u, mine);
+      const int at = pos + __popc(mk & below);
+      if (mine && at < m) {                           // (always, unless another stream changes the weights meanwhile)
+        kept[at] = i + 32 * e + lane;
+        nw[at] = weight_of(k[e]);
       }
-      tie_at += __popc(mt[e]);
+      tie_at += __popc(mt);
       pos += __popc(mk);
     }
   }
-  if (CL) sync();                                     // the others have read this CTA's counts
+  if (CL) cl.barrier_wait();                          // the others have read this CTA's counts
 }
 
 // Rows to other pages: a CTA copies TOK kept tokens, 16-byte pieces, eight of each thread's in flight.
@@ -332,16 +333,12 @@ cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
   const long long most = width < a.w_len ? width : a.w_len;
   const int c = cluster_of(groups, most);
   const long long seg = (most + c - 1) / c;
-  cudaError_t e;
-  if (seg <= MAX_KEYS) {
-    const auto k = c > 1 ? k_select<true, true> : k_select<true, false>;
-    static std::atomic<bool> done[2][MAX_DEVICES];
-    int dev = 0, sms = 0;
-    if ((e = device_sms(dev, sms)) || (e = allow_smem(k, MAX_KEYS * 4, dev, done[c > 1]))) return e;
-    e = launch(k, static_cast<unsigned>(groups * c), NT, static_cast<size_t>(seg) * 4, c, st, a, c);
-  } else {                                            // (the largest cluster)
-    e = launch(k_select<false, true>, static_cast<unsigned>(groups * c), NT, 0, c, st, a, c);
-  }
+  // as many registers as the longest row's keys take: two CTAs to an SM up to 8192 keys
+  const auto k = seg > MAX_KEYS      ? k_select<32, false, true>    // (the largest cluster)
+                 : seg > MAX_KEYS / 2 ? (c > 1 ? k_select<32, true, true> : k_select<32, true, false>)
+                 : seg > MAX_KEYS / 4 ? (c > 1 ? k_select<16, true, true> : k_select<16, true, false>)
+                                      : (c > 1 ? k_select<8, true, true> : k_select<8, true, false>);
+  const cudaError_t e = launch(k, static_cast<unsigned>(groups * c), NT, 0, c, st, a, c);
   if (e != cudaSuccess) return e;
   if (!a.dst_bt) {
     // a CTA per (row, kv head) where they fill the SMs, else a cluster (256 of them: 119 us with one CTA, 127 with two, 138 with

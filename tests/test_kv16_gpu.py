@@ -451,6 +451,16 @@ def test_evict_long(K, in_place, lens, budget):
     check_evict(K, lens, 2, 64, 16, BF, budget, 4, 64, 21, in_place)
 
 
+@pytest.mark.parametrize("levels", [0, 3])                      # weights: random, or of few values (many ties)
+@pytest.mark.parametrize("lens,Hkv,budget", [([4097, 4100, 64] * 25, 2, 2000), ([8200, 50, 8191, 4096] * 19, 2, 1000), ([17000, 900] * 38, 2, 900),
+                                             ([66000], 1, 7000), ([140000, 9, 131073], 2, 6000), ([262200], 1, 262144)])
+def test_evict_rows_of_every_size_class(K, lens, Hkv, budget, levels):
+    W = -(-max(lens) // 16) * 16 + 3
+    g = gen(budget + levels)
+    w = torch.randint(0, levels, (len(lens), Hkv, W), generator=g).float() if levels else torch.rand(len(lens), Hkv, W, generator=g)
+    check_evict(K, lens, Hkv, 64, 16, BF, budget, 4, 100, 31, False, weights=w)
+
+
 def test_evict_ties_infinities_nan_and_signs(K):
     """equal weights go to the lower position; -0 equals +0; NaN is the smallest; negative weights and infinities order"""
     g = gen(22)
