@@ -2,16 +2,18 @@
 //
 // HBM bound: 8 D bytes move per kept (token, kv head) (key and value row, read and written), 4 bytes are read per weight.
 // Two launches:
-//   k_select  a cluster of 1 to 8 CTAs per (row, kv head): the threshold by a radix search over order-preserving keys (four
-//             digits of 8 bits; the CTAs' histograms are added through distributed shared memory), then one scan that writes the
-//             kept positions and their weights;
+//   k_select  a cluster of 1 to 8 CTAs per (row, kv head), the weights' order-preserving keys in registers: the threshold by a
+//             radix search (four digits of 8 bits; the CTAs' histograms are added through distributed shared memory), then the
+//             kept positions and their weights are written in order;
 //   k_copy    (other pages) a CTA per 64 kept tokens, or
 //   k_move    (in place) a cluster per (row, kv head) that moves the rows down step by step: a kept token only moves to a lower
 //             position, so a step's writes hit no row that a later step reads, and one cluster barrier per step is enough.
 //
-// Measured (D 128): 32 rows of up to 4096 tokens x 8 heads to 2048: 101 us, of which the copy 82 (the measured copy rate); one row of
-// 60000 x 8 heads to 7500: 34 us, of which the copy 10 and the selection, eight clusters of eight CTAs that meet six times, most
-// of the rest.  In place: 120 and 54 us (a step's reads and the writes of the step before it overlap, the next one's do not).
+// Measured (D 128): 32 rows of up to 4096 tokens x 8 heads to 2048: 99 us, of which the copy 82 (the measured copy rate); one row of
+// 60000 x 8 heads to 7500: 28.5 us, of which the copy 10 and the selection 14: eight clusters of eight CTAs that meet five times
+// (1.9 us a digit, half of it the barrier and the others' histograms).  With the keys in shared memory instead of registers the
+// selection took 19 us.  In place: 117 and 48 us (a step's reads and the writes of the step before it overlap, the next one's
+// do not).
 #include <cooperative_groups.h>
 
 #include "k16_kernels.h"
@@ -33,6 +35,10 @@ FR_DEVI uint32_t key_of(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 FR_DEVI float weight_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }   // (0: a NaN)
+// one more in a counter of shared memory, under a predicate (a branch around each: the first two passes a fifth longer)
+FR_DEVI void count_if(uint32_t on, uint32_t counter) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %0, 0;\n @p red.shared.add.u32 [%1], 1;\n}\n" ::"r"(on), "r"(counter) : "memory");
+}
 // the n lowest of 32 bits
 FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
@@ -88,13 +94,14 @@ template <int KPT, bool ONCE, bool CL> __global__ void __launch_bounds__(NT, KPT
 #pragma unroll 1
     for (int p = 0; p < PASSES; ++p) {
       const int sh = 32 - DIGIT * (p + 1);
+      const uint32_t h0 = static_cast<uint32_t>(__cvta_generic_to_shared(&hist[p][0]));
       for (int i = i0; i < i1; i += 32 * KPT) {
         if (!ONCE) load(i);
         const uint32_t cand = chosen_from(i), top = p == 0 ? 0u : ~0u << (sh + DIGIT);
 #pragma unroll
         for (int e = 0; e < KPT; ++e) {
           if (i + 32 * e >= i1) break;
-          if ((cand >> e & 1) && ((k[e] ^ T) & top) == 0) atomicAdd(&hist[p][(k[e] >> sh) & (BINS - 1)], 1);
+          count_if(((k[e] ^ T) & top) == 0 ? cand & (1u << e) : 0u, h0 + 4 * ((k[e] >> sh) & (BINS - 1)));
         }
       }
       sync();
@@ -190,19 +197,23 @@ template <int KPT, bool ONCE, bool CL> __global__ void __launch_bounds__(NT, KPT
   const unsigned below = (1u << lane) - 1;
   for (int i = i0; i < i1; i += 32 * KPT) {
     if (!ONCE) load(i), mark(i);
+    if (__any_sync(~0u, mtie != 0)) {                 // of the ties the first left - tie_at are taken
+#pragma unroll 1
+      for (int e = 0; e < KPT; ++e) {
+        const unsigned mt = __ballot_sync(~0u, mtie >> e & 1);
+        if ((mtie >> e & 1) && tie_at + __popc(mt & below) < left) msure |= 1u << e;
+        tie_at += __popc(mt);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < KPT; ++e) {
       if (i + 32 * e >= i1) break;
-      // of the ties the first left - tie_at are taken
-      const unsigned mt = __ballot_sync(~0u, mtie >> e & 1);
-      const bool mine = (msure >> e & 1) || ((mtie >> e & 1) && tie_at + __popc(mt & below) < left);
-      const unsigned mk = __ballot_sync(~0u, mine);
+      const unsigned mk = __ballot_sync(~0u, msure >> e & 1);
       const int at = pos + __popc(mk & below);
-      if (mine && at < m) {                           // (always, unless another stream changes the weights meanwhile)
+      if ((msure >> e & 1) && at < m) {               // (at < m: unless another stream changes the weights meanwhile)
         kept[at] = i + 32 * e + lane;
         nw[at] = weight_of(k[e]);
       }
-      tie_at += __popc(mt);
       pos += __popc(mk);
     }
   }
@@ -316,12 +327,12 @@ template <int D, bool CL> __global__ void __launch_bounds__(MT, 2) k_move(EvictA
   }
 }
 
-// CTAs per (row, kv head): enough to use the SMs, of at least 2048 positions each, and to hold the weights in shared memory.
-// 32 x 4096 x 8 heads: 101 us with one CTA, 131 with four, 174 with eight; 1 x 60000 x 8 heads: 45 with four, 34 with eight, 51 with
-// eight that read the weights again in every pass.
+// CTAs per (row, kv head): as many as the SMs hold at once, of at least 2048 positions each, and enough to hold the weights in
+// registers.  32 x 4096 x 8 heads: 99 us with one CTA, 114 with two, 186 with eight; 16 x 16000 x 8: 41 with one, 42 with two, 52 with
+// four; 4 x 30000 x 8: 27 with two, 21 with four, 23 with eight; 1 x 60000 x 8: 35 with four, 28.5 with eight.
 int cluster_of(long long groups, long long positions) {
   int c = 1;
-  while (c < 8 && ((groups * c < 148 && positions / c > 2048) || positions / c > MAX_KEYS)) c *= 2;
+  while (c < 8 && ((groups * c * 2 <= 148 && positions / c > 2048) || positions / c > MAX_KEYS)) c *= 2;
   return c;
 }
 
@@ -341,8 +352,8 @@ cudaError_t evict(const EvictArgs& a, cudaStream_t st) {
   const cudaError_t e = launch(k, static_cast<unsigned>(groups * c), NT, 0, c, st, a, c);
   if (e != cudaSuccess) return e;
   if (!a.dst_bt) {
-    // a CTA per (row, kv head) where they fill the SMs, else a cluster (256 of them: 119 us with one CTA, 127 with two, 138 with
-    // eight; 8 of them: 211, 138 and 53 us)
+    // a CTA per (row, kv head) where they fill the SMs, else a cluster (256 of them: 117 us with one CTA, 125 with two, 136 with
+    // eight; 8 of them: 206, 134 and 48 us)
     int cm = 1;
     while (cm < 8 && groups * cm < 148 && a.budget / cm > 256) cm *= 2;
     const auto k = a.D == 128 ? (cm > 1 ? k_move<128, true> : k_move<128, false>) : (cm > 1 ? k_move<64, true> : k_move<64, false>);
