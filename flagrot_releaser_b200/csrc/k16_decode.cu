@@ -14,11 +14,12 @@
 //
 // CTA: four consumer warps and a producer warp that fills a ring of 16 KB stages (one block: 32 keys and their values) with
 // two tensor copies each; two CTAs per SM, so that a CTA's start and joins are covered by the other's stream.  A block goes to
-// NT warps, one per tile of TR q heads: one tile of 8 for G up to 8, two of 8 up to 16, two of 16 above.  A weight meets the
+// NT warps, one per tile of TR q heads: one tile of 8 for G up to 8, up to 16 two of 8 (D 128) or one of 16 (D 64), two of 16 above.  A weight meets the
 // values as p = hi + lo, both of the cache's type, with an error of 2^-17 instead of 2^-9: in a tile of 8 the other 8 rows of
 // the second MMA carry lo, at no extra cost; in a tile of 16 lo is a product of its own.  Per head that is a quarter fewer MMAs
 // and half the reads of shared memory: G 32 (64 rows of 4096 tokens, 4 kv heads, D 128) 122 us, with four tiles of 8 157;
-// D 64 43 and 53.  G 16 as one tile of 16: 191 us where two of 8 take 177, for a warp then is too long at a block.
+// D 64 43 and 53.  G 16 as one tile of 16: D 128 191 us where two of 8 take 177, for then all four stages are being worked on;
+// D 64, with eight stages, 109 and 112.
 //
 // Measured (bf16, D 128, G 4, page 16, of the measured copy rate of 6.55 TB/s): 64 rows of up to 4096 tokens 153 us = 0.95; one
 // row of 131072 94 us = 0.87; 32 rows x 1028 visible of 16384 29 us = 0.72; one row of 77 tokens 5 us on the device.  What is
@@ -598,7 +599,7 @@ template <int DT, int D>
 cudaError_t launch_nt(const AttnArgs& a, const CUtensorMap& map, int dev, int grid, int nhg, float* part, float* lse, float* scores, long long ld,
                       cudaStream_t st) {
   if (a.G <= 8) return launch_d<DT, D, 8, 1>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
-  if (a.G <= 16) return launch_d<DT, D, 8, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
+  if (a.G <= 16) return launch_d<DT, D, D == 64 ? 16 : 8, D == 64 ? 1 : 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
   return launch_d<DT, D, 16, 2>(a, map, dev, grid, nhg, part, lse, scores, ld, st);
 }
 
