@@ -14,11 +14,11 @@
 //
 // CTA: four consumer warps and a producer warp that fills a ring of 16 KB stages (one block: 32 keys and their values) with
 // two tensor copies each; two CTAs per SM, so that a CTA's start and joins are covered by the other's stream.  A block goes to
-// NT warps, one per tile of TR q heads: one tile of 8 for G up to 8, up to 16 two of 8 (D 128) or one of 16 (D 64), two of 16 above.  A weight meets the
-// values as p = hi + lo, both of the cache's type, with an error of 2^-17 instead of 2^-9: in a tile of 8 the other 8 rows of
-// the second MMA carry lo, at no extra cost; in a tile of 16 lo is a product of its own.  Per head that is a quarter fewer MMAs
-// and half the reads of shared memory: G 32 (64 rows of 4096 tokens, 4 kv heads, D 128) 122 us, with four tiles of 8 157;
-// D 64 43 and 53.  G 16 as one tile of 16: D 128 191 us where two of 8 take 177, for then all four stages are being worked on;
+// NT warps, one per tile of TR q heads: one tile of 8 for G up to 8, up to 16 two of 8 (D 128) or one of 16 (D 64), two of 16
+// above.  A weight meets the values as p = hi + lo, both of the cache's type, with an error of 2^-17 instead of 2^-9: in a tile
+// of 8 the other 8 rows of the second MMA carry lo, at no extra cost; in a tile of 16 lo is a product of its own.  Per head that
+// is a quarter fewer MMAs and half the reads of shared memory: G 32 (64 rows of 4096 tokens, 4 kv heads, D 128) 122 us, with
+// four tiles of 8 157; D 64 43 and 53.  G 16 as one tile of 16: D 128 191 us where two of 8 take 177, for then all four stages are being worked on;
 // D 64, with eight stages, 109 and 112.
 //
 // Measured (bf16, D 128, G 4, page 16, of the measured copy rate of 6.55 TB/s): 64 rows of up to 4096 tokens 153 us = 0.95; one

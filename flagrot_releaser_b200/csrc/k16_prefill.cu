@@ -25,7 +25,8 @@
 // 3900 cycles, 2500 of them tensor (the N = 64 products of the halves cost 48 cycles instead of 32); the rest is latency of
 // the one softmax warp per tile and scheduler.  Measured and not kept: a polynomial 2^x for part of the weights (the MUFU is
 // half idle), two threads per row (104 registers a thread: spills), whole 128-key S tiles (the same time, windows 8 % slower),
-// turns between the tiles' exponentials (the same), output by warps of its own (2 % and 8 % slower).
+// turns between the tiles' exponentials (the same), output by warps of its own (2 % and 8 % slower), one loop over the halves that
+// a tile needs, with the half chosen at run time (3 % slower).
 #include "k16_kernels.h"
 #include "k16_launch.cuh"
 #include "k16_tma.cuh"
