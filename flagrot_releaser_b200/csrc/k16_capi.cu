@@ -31,6 +31,18 @@ int check_cache(const void* pool, long long num_pages, const int* bt, long long 
   if (B > 0 && (!pool || !al16(pool) || !lens || (bt_width > 0 && !bt))) return -3;
   return 0;
 }
+// whether the n 4-byte entries at x share any with `rows` rows of `width` such entries, `stride` entries apart, at p
+bool meets(const void* x, long long n, const void* p, long long rows, long long stride, long long width) {
+  const long long a = static_cast<long long>(reinterpret_cast<uintptr_t>(x)) - static_cast<long long>(reinterpret_cast<uintptr_t>(p));
+  if (!p || n <= 0 || rows <= 0 || width <= 0) return false;
+  if (stride <= width) {                                 // no gaps: one row
+    width += (rows - 1) * stride;
+    rows = 1;
+    stride = width;
+  }
+  const long long k = a < 4 * width ? 0 : (a - 4 * width) / (4 * stride) + 1;   // the first row that ends behind a
+  return k < rows && 4 * k * stride < a + 4 * n;
+}
 Cache make_cache(const void* pool, long long num_pages, const int* bt, long long bt_stride, int bt_width, const int* lens, int Hkv,
                  int page) {
   Cache c;
@@ -169,6 +181,15 @@ int k16_evict(const void* pool, long long num_pages, const int* block_table, lon
     a.dst = static_cast<uint16_t*>(const_cast<void*>(pool));
     a.dst_pages = num_pages;
   }
+  // Some CTAs write results while others still read the inputs (a row's heads and a cluster's CTAs run apart).
+  const long long groups = static_cast<long long>(B) * Hkv, w_span = w_len > 0 ? (B - 1) * w_bs + (Hkv - 1) * w_hs + w_len : 0;
+  const void* result[3] = {kept, new_lens, new_weights};
+  const long long count[3] = {groups * budget, B, groups * nw_len};
+  for (int i = 0, j = 1; i < 3; ++i, j = (j + 1) % 3)
+    if (meets(result[i], count[i], seq_lens, 1, B, B) || meets(result[i], count[i], weights, 1, w_span, w_span) ||
+        meets(result[i], count[i], block_table, B, bt_stride, bt_width) || meets(result[i], count[i], dst_table, B, dst_stride, dst_width) ||
+        meets(result[i], count[i], result[j], 1, count[j], count[j]))
+      return -3;
   a.c = make_cache(pool, num_pages, block_table, bt_stride, bt_width, seq_lens, Hkv, page);
   a.B = B;
   a.D = D;

@@ -66,7 +66,8 @@ int k16_prefill(int dtype, const void* q, long long q_ts, int T, const int* cu_q
  * the others, the budget - sinks - recent with the largest weights (ties: the lower position; NaN counts as the smallest),
  * in their order.  weights fp32 as in k16_attn (len is also taken within w_len = its entries per row).
  * kept int32 [B, Hkv, budget]: the kept positions, then -1; new_lens int32 [B] = min(len, budget); new_weights fp32
- * [B, Hkv, nw_len] (contiguous, nw_len >= budget): the kept tokens' weights, then zeros.
+ * [B, Hkv, nw_len] (contiguous, nw_len >= budget): the kept tokens' weights, then zeros.  The three results overlap neither one
+ * another nor seq_lens, weights (from their first entry to their last) and the tables: -3 otherwise.
  * dst_table null: the kept rows move to the front of the row's own pages (no page may belong to two rows).  Else they are
  * copied to the pages of dst_table [B, dst_width] in dst_pool (distinct pages, dst_width * page >= budget; entries outside
  * [0, dst_pages) are not written), which share no page with the ones that are read; slots behind the kept rows are left as

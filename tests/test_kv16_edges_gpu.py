@@ -1,0 +1,72 @@
+"""The 16-bit paged cache on a GPU in calls that the documentation allows and test_kv16_gpu.py does not make.  Definitions and
+tolerances are the ones of that file and of _kv16.py."""
+import pytest
+import torch
+
+from tests import _kv16 as R
+from tests.test_kv16_gpu import BF, DEV, gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K():
+    from flagrot_releaser_b200 import kv16
+    kv16.lib()
+    yield kv16
+    assert kv16.device_status() == 0
+
+
+def carve(shapes):
+    """tensors one right behind the other in one buffer (4-byte types)"""
+    sizes = [torch.Size(s).numel() for s, _ in shapes]
+    buf, out, at = torch.zeros(sum(sizes), dtype=torch.int32, device=DEV), [], 0
+    for (s, t), n in zip(shapes, sizes):
+        out.append(buf[at:at + n].view(t).view(s))
+        at += n
+    return out
+
+
+@pytest.mark.parametrize("order", [[0, 1, 2, 3, 4, 5], [5, 3, 1, 4, 2, 0], [2, 4, 0, 5, 1, 3]])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_takes_tensors_that_touch(K, order, in_place):
+    """lengths, weights, table and the three results side by side in one buffer, in any order, are not an overlap"""
+    g = gen(61)
+    lens, Hkv, page, budget = [100, 7, 333], 2, 16, 64
+    pool, table, _ = R.make_cache(lens, Hkv, 64, page, BF, g, poison=False)
+    W = table.shape[1] * page
+    shapes = [((3,), torch.int32), ((3, Hkv, W), torch.float32), (tuple(table.shape), torch.int32), ((3, Hkv, budget), torch.int32),
+              ((3,), torch.int32), ((3, Hkv, budget), torch.float32)]
+    t = [None] * 6
+    for i, x in zip(order, carve([shapes[i] for i in order])):
+        t[i] = x
+    ln, w, bt, kept, nl, nw = t
+    ln.copy_(torch.tensor(lens)), bt.copy_(table), w.copy_(torch.rand(w.shape, generator=g))
+    keep = [x.clone() for x in (ln, w, bt)]
+    kw = {} if in_place else dict(dst_pool=torch.zeros_like(pool), dst_table=torch.arange(12, dtype=torch.int32, device=DEV).view(3, 4))
+    K.evict(pool, bt, ln, w, budget, 4, 16, kept, nl, nw, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(keep, (ln, w, bt)))
+    for b, n in enumerate(lens):
+        m = min(n, budget)
+        ref = R.evict_ref(w[b], n, budget, 4, 16)
+        assert int(nl[b]) == m and [x[:m] for x in kept[b].tolist()] == ref
+        assert torch.equal(nw[b, :, :m], w[b].gather(1, torch.tensor(ref, device=DEV)))
+
+
+def test_evict_takes_results_in_the_gaps_of_a_table(K):
+    """a table whose rows lie far apart; the results lie between them"""
+    g = gen(62)
+    lens, Hkv, page, budget = [100, 90], 1, 16, 32
+    pool, table, ln = R.make_cache(lens, Hkv, 64, page, BF, g, poison=False)
+    width, gap = table.shape[1], 2 * budget + 2
+    buf = torch.zeros(2, width + 2 * gap, dtype=torch.int32, device=DEV)
+    bt = buf[:, :width]
+    bt.copy_(table)
+    between = buf.view(-1)[width:]
+    kept, nl = between[:2 * budget].view(2, 1, budget), between[2 * budget:2 * budget + 2]
+    nw = between[gap:gap + 2 * budget].view(torch.float32).view(2, 1, budget)
+    w = torch.rand(2, Hkv, width * page, generator=g).to(DEV)
+    K.evict(pool, bt, ln, w, budget, 2, 8, kept, nl, nw)
+    assert torch.equal(bt, table) and nl.tolist() == [budget, budget]
+    for b, n in enumerate(lens):
+        assert kept[b].tolist() == R.evict_ref(w[b], n, budget, 2, 8)
