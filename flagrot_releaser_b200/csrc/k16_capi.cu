@@ -63,6 +63,7 @@ extern "C" {
 int k16_abi_version(void) { return 1; }
 const char* k16_last_error(void) { return g_err; }
 int k16_device_status(void) {
+  if (fail(cudaDeviceSynchronize())) return -1;   // the copies below do not wait for non-blocking streams
   const int d = decode_status();
   return d ? d : prefill_status();
 }

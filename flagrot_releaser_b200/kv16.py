@@ -86,7 +86,8 @@ def chunk_bytes(page: int, D: int = 128) -> int:
 
 
 def device_status() -> int:
-    """0, or the source line of a bounded device-side wait that gave up (synchronises)."""
+    """0, or the source line of a bounded device-side wait that gave up; -1 when the device cannot be asked.  Waits for every
+    stream of the current device: not during a capture."""
     return lib().k16_device_status()
 
 

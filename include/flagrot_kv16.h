@@ -24,7 +24,8 @@ extern "C" {
 
 int k16_abi_version(void);
 const char* k16_last_error(void);
-/* 0, or the source line of a bounded device-side wait that gave up (sticky; synchronises the device). */
+/* 0, or the source line of a bounded device-side wait that gave up (sticky); -1 when the device cannot be asked.  Waits for
+ * everything launched on the current device, on every stream: not during a capture. */
 int k16_device_status(void);
 /* bytes per (page, kv head): 4 * page * D */
 int k16_chunk_bytes(int page, int D);

@@ -70,3 +70,15 @@ def test_evict_takes_results_in_the_gaps_of_a_table(K):
     assert torch.equal(bt, table) and nl.tolist() == [budget, budget]
     for b, n in enumerate(lens):
         assert kept[b].tolist() == R.evict_ref(w[b], n, budget, 2, 8)
+
+
+def test_device_status_waits_for_side_streams(K):
+    """the status is that of the calls made so far, on streams that the default stream does not wait for too"""
+    K.device_status()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(400_000_000)                     # a fifth of a second
+    assert not any(s.query() for s in streams), "the streams ended too soon for this test"
+    assert K.device_status() == 0
+    assert all(s.query() for s in streams)
