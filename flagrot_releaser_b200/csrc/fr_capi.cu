@@ -211,6 +211,7 @@ int fr_dyn_writer_stats(unsigned long long* out2, int reset) { return fr::dyn_wr
 void fr_dyn_writer_exact_only(int on) { fr::dyn_writer_exact_only(on); }
 
 int fr_device_status() {
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;   // the copies below do not wait for non-blocking streams
   const int d = fr::decode_status();
   if (d != 0) return d;
   const int w = fr::writer_status();

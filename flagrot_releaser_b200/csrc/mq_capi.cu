@@ -302,6 +302,7 @@ int frmq_smem_bytes() { return TQMap<4, 3>::TOTAL; }
 /* no counterpart in the reference: 0, or the source line of a bounded device-side wait that gave up (sticky) */
 int frmq_device_status() {
   int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;   // the copy below does not wait for non-blocking streams
   cudaMemcpyFromSymbol(&v, g_mq_status, sizeof(int));
   return v;
 }

@@ -143,7 +143,8 @@ int fr_xchg_merge(const float* part, void* const* bufs, int rank, int R, int row
 int fr_xchg_selftest(const float* const* parts, void* const* bufs, int R, int rows, void* const* outs, int out_fp32,
                      void* stream);
 
-/* 0, or the source line of a bounded device-side wait that gave up (sticky; synchronises the device). */
+/* 0, or the source line of a bounded device-side wait that gave up (sticky; synchronises the device, every stream of it);
+ * -1 when the device cannot be asked (a capture, no device). */
 int fr_device_status(void);
 
 /* Bulk key writer of fr_cb_write / fr_cb_write3 (more than 4096 (token, kv head) pairs per call): the head choice

@@ -19,7 +19,7 @@ int frmq_abi_version(void);
 const char* frmq_last_error(void);
 int frmq_smem_bytes(void);
 /* no counterpart in the reference: 0, or the source line of a bounded device-side wait that gave up (sticky;
- * synchronises the device) */
+ * synchronises the device, every stream of it); -1 when the device cannot be asked (a capture, no device) */
 int frmq_device_status(void);
 
 /* q (bf16, or fp32 when q_fp32; row stride q_ts elements; rows idx[0..m) or 0..m) -> FP16 [m, Hq, 128] in the keys' stored
