@@ -36,6 +36,8 @@ constexpr int BLK = 32;                  // keys per block
 constexpr int MAX_CTAS = 2 * 148;        // partial slots of the workspace: two per CTA
 constexpr int MAX_GT = 32;               // q heads per segment
 constexpr float LAZY = 8.f;              // the softmax reference moves when a score exceeds it by more than this (log2)
+// the reference before the first score: finite, so that a weight against it is 0 and not NaN where every score is -inf
+constexpr float NO_REF = -3.402823466e38f;
 
 __device__ int g_status;
 
@@ -157,6 +159,10 @@ FR_DEVI void wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort, in
 }
 #define k16_wait(bar, parity, abort) wait_at(bar, parity, abort, __LINE__)
 
+// a row whose scores are all -inf has no weights: zeros, and nothing added to its sums
+FR_DEVI float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+template <int DT> FR_DEVI float log_sum(float ref, float sum) { return sum == 0.f ? INFINITY : ref + log2f(sum) - (DT == 1 ? 6.f : 0.f); }
+
 // The pieces of CTAs c0 .. c1 of the segment that begins at f0, in order: four dims of a head per thread, eight pieces in flight;
 // few heads: the threads also share the pieces, and their sums meet in shared memory (scr).
 template <int DT, int D>
@@ -165,12 +171,12 @@ FR_DEVI void join(const AttnArgs& a, const float* part, long long quota, long lo
   constexpr int NTH = 32 * NW, IN = 8;
   const int cols = heads * (D / 4), tid = threadIdx.x, sets = max(NTH / cols, 1), stride = sets > 1 ? cols * sets : NTH;
   const auto finish = [&](int col, float M, float L, float4 v) {
-    const float inv = 1.f / L;
+    const float inv = inverse(L);
     uint2 r;
     r.x = Elem<DT>::pack(v.x * inv, v.y * inv);
     r.y = Elem<DT>::pack(v.z * inv, v.w * inv);
     *reinterpret_cast<uint2*>(out + 4 * col) = r;              // (col = head * D / 4 + dims)
-    if (lse && col % (D / 4) == 0) lse[col / (D / 4)] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
+    if (lse && col % (D / 4) == 0) lse[col / (D / 4)] = log_sum<DT>(M, L);
   };
   for (int i = tid; i < (sets > 1 ? stride : cols); i += stride) {
     const int col = i % cols, set = i / cols, hh = col / (D / 4), d = 4 * (col - hh * (D / 4));
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
     }
     float o[ND][4], ref[R], l[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) ref[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < R; ++r) ref[r] = NO_REF, l[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     const int cnt = wk.k1 - wk.k0;
@@ -445,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 2));
         moves |= mx[r] > ref[r] + LAZY;
       }
-      if (__any_sync(~0u, moves)) {                            // (the first block: ref = -inf)
+      if (__any_sync(~0u, moves)) {                            // (the first block: ref = NO_REF)
         float f[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -525,9 +531,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_decode(const __grid_constant__ A
         v.y = fmaf(f, y.y, v.y);
       }
       if (c0 == c1) {
-        const float inv = 1.f / L;
+        const float inv = inverse(L);
         reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + wk.b * a.o_bs + (hq0 + hh) * D)[d >> 1] = Elem<DT>::pack(v.x * inv, v.y * inv);
-        if (lse && d == 0) lse[static_cast<long long>(wk.b) * Hq + hq0 + hh] = M + log2f(L) - (DT == 1 ? 6.f : 0.f);
+        if (lse && d == 0) lse[static_cast<long long>(wk.b) * Hq + hq0 + hh] = log_sum<DT>(M, L);
       } else {
         *reinterpret_cast<float2*>(slot + hh * D + d) = v;
         if (d == 0) *reinterpret_cast<float2*>(slot + GT * D + 2 * hh) = make_float2(M, L);

@@ -45,7 +45,8 @@ long long k16_ws_tickets(int rows, int Hkv, int G, long long new_tokens);
 
 /* Attention of one new token per row.  q [B, G*Hkv, D] (row stride q_bs elements), key j of row b is visible when j < len
  * and (window <= 0 or j >= len - window or j < sinks); qscale = softmax scale * log2(e); out [B, G*Hkv*D] (row stride
- * o_bs); q and out rows 16-byte aligned.  A row that sees no key is written as zeros.
+ * o_bs); q and out rows 16-byte aligned.  A row that sees no key, or only keys whose score is -inf, is written as zeros (and adds
+ * nothing to weights); beside others a key whose score is -inf has weight 0.  The same in k16_prefill.
  * weights fp32 (or null): weights[b * w_bs + h * w_hs + j] += the softmax weights of visible key j summed over the G heads of
  * kv head h; other entries are left as they are.  Each row needs at least bt_width * page entries, rows of its own. */
 int k16_attn(int dtype, const void* q, long long q_bs, const void* pool, long long num_pages, const int* block_table,

@@ -1,10 +1,12 @@
 """The 16-bit paged cache on a GPU in calls that the documentation allows and test_kv16_gpu.py does not make.  Definitions and
 tolerances are the ones of that file and of _kv16.py."""
+import math
+
 import pytest
 import torch
 
 from tests import _kv16 as R
-from tests.test_kv16_gpu import BF, DEV, gen
+from tests.test_kv16_gpu import BF, DEV, FP, bound, check_attn, gen, queries, run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +84,63 @@ def test_device_status_waits_for_side_streams(K):
     assert not any(s.query() for s in streams), "the streams ended too soon for this test"
     assert K.device_status() == 0
     assert all(s.query() for s in streams)
+
+
+def barred(lens, first, Hkv, D, page, dtype, g, value):
+    """a cache whose rows' first `first` keys are barred by `value` in their first channel, which every query multiplies by a
+    positive number"""
+    pool, bt, ln = R.make_cache(lens, Hkv, D, page, dtype, g)
+    pc = pool.cpu()
+    for b, n in enumerate(lens):
+        for j in range(min(first, n)):
+            pc[int(bt[b, j // page]), :, 0, j % page, 0] = value
+    return pc.to(DEV), bt, ln
+
+
+@pytest.mark.parametrize("value", [-math.inf, "lowest"])
+@pytest.mark.parametrize("first", [1, 31, 32, 33, 64, 200, 1000])
+@pytest.mark.parametrize("G,D,page,dtype", [(4, 128, 16, BF), (1, 64, 64, FP), (12, 64, 16, BF), (12, 128, 32, FP), (24, 128, 16, BF)])
+def test_attn_keys_barred_by_infinite_scores(K, G, D, page, dtype, first, value):
+    """keys whose score is -inf have weight 0, however many of them come first; a row that has no others gives zeros and adds
+    nothing to the weights.  The type's lowest value does the same beside other keys (bf16: the product passes the 32-bit
+    range; fp16: scores below -40 000)."""
+    g = gen(71)
+    lens = [5, 32, 40, 64, 300, 1111, 9000]
+    pool, bt, ln = barred(lens, first, 2, D, page, dtype, g, -math.inf)
+    given = pool if value != "lowest" else torch.where(pool == -math.inf, torch.full((), torch.finfo(dtype).min, dtype=dtype, device=DEV), pool)
+    q = queries(len(lens), 2 * G, D, dtype, g)
+    q[..., 0] = q[..., 0].abs() + 4
+    w0 = torch.rand(len(lens), 2, bt.shape[1] * page, generator=g).to(DEV)
+    w1 = w0.clone()
+    qs = R.LOG2E / math.sqrt(D)
+    for w in (w1, None):
+        out = run_attn(K, q, given, bt, ln, qs, weights=w)
+        none = ln <= first
+        if value != "lowest":
+            assert bool((out[none] == 0).all())
+            if w is not None:
+                assert torch.equal(w0[none], w1[none])
+        assert bool(torch.isfinite(out).all())
+        some = (~none).nonzero().flatten()
+        check_attn(out[some], q[some], pool, bt[some], ln[some], qs, 0, 0, *((w0[some], w1[some]) if w is not None else ()))
+
+
+@pytest.mark.parametrize("first", [1, 64, 65, 300])
+@pytest.mark.parametrize("G,D,page,dtype", [(4, 128, 16, BF), (12, 64, 64, FP)])
+def test_prefill_keys_barred_by_infinite_scores(K, G, D, page, dtype, first):
+    g = gen(72)
+    lens, new = [5, 40, 300, 1111, 9000], [5, 1, 200, 333, 9]
+    pool, bt, ln = barred(lens, first, 2, D, page, dtype, g, -math.inf)
+    T = sum(new)
+    q = queries(T, 2 * G, D, dtype, g)
+    q[..., 0] = q[..., 0].abs() + 4
+    cu = torch.tensor([0] + [sum(new[:i + 1]) for i in range(len(new))], dtype=torch.int32, device=DEV)
+    ws, qs = K.Workspace(len(lens), 2, G, D, bt.shape[1] * page, DEV, new_tokens=T), R.LOG2E / math.sqrt(D)
+    out = torch.full((T, 2 * G * D), 7.0, dtype=dtype, device=DEV)
+    K.prefill(q, cu, pool, bt, ln, out, qs, ws=ws)
+    for b, (n, m) in enumerate(zip(lens, new)):
+        k, v = R.rows_of(pool, bt[b], n)
+        s = slice(int(cu[b]), int(cu[b + 1]))
+        o, _, A, S = R.attend(q[s].double(), k, v, torch.arange(n - m, n), qs, 0, 0)
+        err = (out[s].view(m, 2 * G, D).double() - o).abs()
+        assert bool((err <= bound(o, A, S, D, n, dtype, True)).all()), (b, n, m)
