@@ -56,6 +56,8 @@ struct Item {
   int k0, k1;                            // ... of which this item takes [k0, k1)
   int ns, part, slot, stride;            // pieces of the pair, this one's number and workspace slot, slots between pieces
   FR_DEVI int block(int k) const { return k < nsb ? k : wb + k - nsb; }
+  // the pair's queries see nothing of [sinks, unseen)
+  FR_DEVI int unseen(int window, int sinks) const { return Span(max(pos0, 0), window, sinks).lo; }
 };
 // the tokens of one tile, as positions [pa, pb]
 struct Tile {
@@ -422,6 +424,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
       if (!k16_wait(qfull, qc & 1)) break;
       ++qc;
       tc5::fence_after_sync();
+      const int unseen = it.unseen(a.window, a.sinks);
+      bool dirty = false;                                      // block k - 1 holds values that no query of the pair sees
       int was = 0;                                             // bit c: the tile needs half c of V(k - 1)
       uint32_t begun = 0;                                      // its O has begun
       int kbv = 0;                                             // first key of block k - 1
@@ -433,11 +437,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         if (k > it.k0) {
           if (!(run = k16_wait(full + 8 * st, ph))) break;
           if (++st == STAGES) st = 0, ph ^= 1;
-          if (was && kbv + BN > it.len) {       // values behind the sequence: 0 * NaN would be NaN
-            for (int j = (it.len - kbv) * 8 + lane; j < BN * 8; j += 32)
+          // Values that no query of the pair sees become zeros, whatever the cache holds there: 0 * NaN would be NaN.  (Both
+          // tiles' warps write them: the same zeros, each before its own product.)
+          if (dirty) {
+            int j0 = min(max(a.sinks - kbv, 0), BN), j1 = min(unseen - kbv, BN);   // behind the window, then behind the sequence
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+#pragma unroll 1
+              for (int j = j0 * 8 + lane; j < j1 * 8; j += 32)
 #pragma unroll
-              for (int x = 0; x < HALVES; ++x)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + j * 16), "r"(0) : "memory");
+                for (int x = 0; x < HALVES; ++x)
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(sv + x * BN * 128 + j * 16), "r"(0) : "memory");
+              j0 = min(it.len - kbv, BN);
+              j1 = BN;
+            }
             tc5::fence_async_smem();
             __syncwarp();
           }
@@ -477,6 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prefill(const __grid_constant__ 
         }
         if (!run) break;
         was = now, kbv = kb;
+        dirty = now && (kb + BN > it.len || kb < unseen);
       }
     }
   } else {                                                     // --------------------------------------------------- softmax

@@ -183,7 +183,8 @@ def prefill(q, cu_q, pool, block_table, seq_lens, out, qscale, window=0, sinks=0
     """q [T, G Hkv, D] -> out [T, G Hkv D], rows 16-byte aligned: row b's new tokens are rows cu_q[b] .. cu_q[b + 1] (int32
     [B + 1]) and the last ones of its seq_lens[b] cached tokens (their keys and values are in the pages already).  The token
     at position p sees key j <= p when window <= 0 or j > p - window or j < sinks; one at a negative position gives zeros;
-    rows of out that belong to no sequence are left as they are.  The cached rows within seq_lens must be finite.  ws: a
+    rows of out that belong to no sequence are left as they are.  Cached rows that none of a sequence's new tokens sees may
+    hold anything (their pages may belong to others by now); the values of those that some see must be finite.  ws: a
     Workspace made with new_tokens."""
     npg, Hkv, page, D = _pool_ok(pool)
     T, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)

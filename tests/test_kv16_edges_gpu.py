@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import _kv16 as R
-from tests.test_kv16_gpu import BF, DEV, FP, bound, check_attn, gen, queries, run_attn
+from tests.test_kv16_gpu import BF, DEV, FP, bound, check_attn, check_prefill, gen, queries, run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,52 @@ def test_prefill_keys_barred_by_infinite_scores(K, G, D, page, dtype, first):
         o, _, A, S = R.attend(q[s].double(), k, v, torch.arange(n - m, n), qs, 0, 0)
         err = (out[s].view(m, 2 * G, D).double() - o).abs()
         assert bool((err <= bound(o, A, S, D, n, dtype, True)).all()), (b, n, m)
+
+
+def prefill_hidden(K, lens, new, Hkv, G, D, page, dtype, window, sinks, seed, give_back):
+    """prefill over a cache whose rows that none of the new tokens sees (behind the first one's window, no sinks) hold NaN and
+    infinities, keys and values; give_back: the pages that hold only such rows belong to someone else's NaN, or to no pool page"""
+    g = gen(seed)
+    pool, bt, ln = R.make_cache(lens, Hkv, D, page, dtype, g)
+    pc, table = pool.cpu(), bt.cpu()
+    for b, (n, m) in enumerate(zip(lens, new)):
+        lo = max(max(n - m, 0) + 1 - window, 0)
+        for j in range(sinks, min(lo, n)):
+            pc[int(table[b, j // page]), :, :, j % page] = (math.nan, math.inf, -math.inf)[j % 3]
+        if give_back:
+            for i in range(-(-sinks // page), lo // page):
+                table[b, i] = (-1, pool.shape[0] + 7, int(bt[b, -1]))[i % 3] if i % 4 else table[b, i]
+    given, clean = pc.to(DEV), pool
+    T = sum(new)
+    q = queries(T, G * Hkv, D, dtype, g, pad=1)
+    cu = torch.tensor([0] + [sum(new[:i + 1]) for i in range(len(new))], dtype=torch.int32, device=DEV)
+    ws, qs = K.Workspace(len(lens), Hkv, G, D, bt.shape[1] * page, DEV, new_tokens=T), R.LOG2E / math.sqrt(D)
+    out = torch.full((T, Hkv * G * D), 7.0, dtype=dtype, device=DEV)
+    K.prefill(q, cu, given, table.to(DEV), ln, out, qs, window=window, sinks=sinks, ws=ws)
+    for b, (n, m) in enumerate(zip(lens, new)):
+        k, v = R.rows_of(clean, bt[b], n)
+        hidden = max(m - n, 0)
+        s = slice(int(cu[b]) + hidden, int(cu[b + 1]))
+        assert bool((out[int(cu[b]):s.start] == 0).all())
+        if s.start < s.stop:
+            o, _, A, S = R.attend(q[s].double(), k, v, torch.arange(n - m + hidden, n), qs, window, sinks)
+            err = (out[s].view(-1, Hkv * G, D).double() - o).abs()
+            assert bool((err <= bound(o, A, S, D, n, dtype, True)).all()), (b, n, m)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 4), (64, 0), (100, 1), (100, 70), (128, 128), (129, 130), (300, 4), (1000, 4)])
+@pytest.mark.parametrize("G,D,page,dtype", [(4, 128, 16, BF), (6, 64, 32, FP), (4, 128, 64, FP), (3, 64, 128, BF), (1, 128, 128, BF)])
+@pytest.mark.parametrize("give_back", [False, True])
+def test_prefill_rows_that_no_new_token_sees_may_hold_anything(K, window, sinks, G, D, page, dtype, give_back):
+    prefill_hidden(K, [700, 90, 1300, 513, 20, 3000], [200, 20, 333, 1, 30, 2], 2, G, D, page, dtype, window, sinks, window + sinks + D, give_back)
+
+
+def test_prefill_long_cache_behind_a_window_may_hold_anything(K):
+    prefill_hidden(K, [20000, 9000], [70, 600], 1, 4, 128, 16, BF, 4096, 4, 5, True)
+    prefill_hidden(K, [20000, 9000], [70, 600], 2, 8, 64, 64, FP, 777, 130, 6, True)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 4), (64, 0), (100, 33), (129, 130), (300, 1), (5000, 4)])
+@pytest.mark.parametrize("G,D,page,dtype", [(4, 128, 64, FP), (4, 64, 128, BF), (2, 128, 128, BF)])
+def test_prefill_window_and_sinks_over_large_pages(K, window, sinks, G, D, page, dtype):
+    check_prefill(K, [700, 90, 1300, 513], [700, 20, 333, 1], 2, G, D, page, dtype, window, sinks, window + sinks)
