@@ -330,9 +330,10 @@ template <int D, bool CL> __global__ void __launch_bounds__(MT, 2) k_move(EvictA
 // CTAs per (row, kv head): as many as the SMs hold at once, of at least 2048 positions each, and enough to hold the weights in
 // registers.  32 x 4096 x 8 heads: 99 us with one CTA, 114 with two, 186 with eight; 16 x 16000 x 8: 41 with one, 42 with two, 52 with
 // four; 4 x 30000 x 8: 27 with two, 21 with four, 23 with eight; 1 x 60000 x 8: 35 with four, 28.5 with eight.
+// (20 x 32769 x 4, one position more than two CTAs' registers hold: 55 with four, 73 with two that read the weights in every pass.)
 int cluster_of(long long groups, long long positions) {
   int c = 1;
-  while (c < 8 && ((groups * c * 2 <= 148 && positions / c > 2048) || positions / c > MAX_KEYS)) c *= 2;
+  while (c < 8 && ((groups * c * 2 <= 148 && positions / c > 2048) || (positions + c - 1) / c > MAX_KEYS)) c *= 2;
   return c;
 }
 

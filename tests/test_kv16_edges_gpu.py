@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import _kv16 as R
-from tests.test_kv16_gpu import BF, DEV, FP, bound, check_attn, check_prefill, gen, queries, run_attn
+from tests.test_kv16_gpu import BF, DEV, FP, bound, check_attn, check_evict, check_prefill, gen, queries, run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +193,12 @@ def test_prefill_long_cache_behind_a_window_may_hold_anything(K):
 @pytest.mark.parametrize("G,D,page,dtype", [(4, 128, 64, FP), (4, 64, 128, BF), (2, 128, 128, BF)])
 def test_prefill_window_and_sinks_over_large_pages(K, window, sinks, G, D, page, dtype):
     check_prefill(K, [700, 90, 1300, 513], [700, 20, 333, 1], 2, G, D, page, dtype, window, sinks, window + sinks)
+
+
+@pytest.mark.parametrize("positions", [32768, 32769, 49153, 65537, 131073])
+def test_evict_around_the_sizes_where_clusters_grow(K, positions):
+    """80 groups: a cluster grows where its CTAs' registers no longer hold the weights, by rounding up"""
+    lens = [positions, 40, positions - 1, 33] + [5] * 36
+    w = torch.rand(40, 2, positions, generator=gen(positions))
+    w[2] = torch.randint(0, 3, (2, positions), generator=gen(1)).float()
+    check_evict(K, lens, 2, 64, 16, BF, 3000, 4, 100, 33, False, weights=w)
