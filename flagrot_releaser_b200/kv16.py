@@ -206,8 +206,10 @@ def evict(pool, block_table, seq_lens, weights, budget, sinks, recent, kept, new
           dst_table=None):
     """Of every (row, kv head) with more than `budget` cached tokens keeps the first `sinks`, the last `recent` and the
     budget - sinks - recent others with the largest weights (fp32 [B, Hkv, W], as attn sums them; ties: the lower position;
-    NaN counts as the smallest), in their order.  kept int32 [B, Hkv, budget]: their positions, then -1; new_lens int32 [B] =
-    min(len, budget); new_weights fp32 [B, Hkv, >= budget]: their weights, then zeros (it must not overlap weights).
+    NaN counts as the smallest), in their order.  A row is taken as min(len, W) tokens long: with W below its length the newest
+    ones are dropped, so give weights as wide as attn wants them (W >= width * page) to keep every one.  kept int32 [B, Hkv,
+    budget]: the kept positions, then -1; new_lens int32 [B] = min(len, W, budget); new_weights fp32 [B, Hkv, >= budget]: the
+    kept tokens' weights, then zeros.  The three results overlap neither one another nor seq_lens, weights and the tables.
     Without dst_table the rows move to the front of the row's own pages (pages must not be shared between rows); with
     it they are copied to the pages of dst_table in dst_pool (default: pool), which must not be among the pages read."""
     npg, Hkv, page, D = _pool_ok(pool)

@@ -68,8 +68,9 @@ int k16_prefill(int dtype, const void* q, long long q_ts, int T, const int* cu_q
 
 /* Evicts: of every (row, kv head) with more than `budget` cached tokens keeps the first `sinks`, the last `recent` and, of
  * the others, the budget - sinks - recent with the largest weights (ties: the lower position; NaN counts as the smallest),
- * in their order.  weights fp32 as in k16_attn (len is also taken within w_len = its entries per row).
- * kept int32 [B, Hkv, budget]: the kept positions, then -1; new_lens int32 [B] = min(len, budget); new_weights fp32
+ * in their order.  weights fp32 as in k16_attn, of w_len entries per row; len is taken within w_len (the newest tokens of a row
+ * that is longer are dropped).
+ * kept int32 [B, Hkv, budget]: the kept positions, then -1; new_lens int32 [B] = min(len, w_len, budget); new_weights fp32
  * [B, Hkv, nw_len] (contiguous, nw_len >= budget): the kept tokens' weights, then zeros.  The three results overlap neither one
  * another nor seq_lens, weights (from their first entry to their last) and the tables: -3 otherwise.
  * dst_table null: the kept rows move to the front of the row's own pages (no page may belong to two rows).  Else they are

@@ -202,3 +202,123 @@ def test_evict_around_the_sizes_where_clusters_grow(K, positions):
     w = torch.rand(40, 2, positions, generator=gen(positions))
     w[2] = torch.randint(0, 3, (2, positions), generator=gen(1)).float()
     check_evict(K, lens, 2, 64, 16, BF, 3000, 4, 100, 33, False, weights=w)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_takes_rows_as_long_as_their_weights(K, in_place):
+    """weights of 100 entries: longer rows lose their newest tokens, within the budget and above it"""
+    w = torch.rand(4, 2, 100, generator=gen(81))
+    check_evict(K, [160, 90, 120, 101], 2, 64, 16, BF, 40, 4, 8, 82, in_place, weights=w)
+    check_evict(K, [160, 90, 120, 101], 2, 64, 16, BF, 110, 4, 8, 83, in_place, weights=w)
+
+
+@pytest.mark.parametrize("D,page,dtype", [(128, 16, BF), (128, 64, FP), (128, 128, BF), (64, 32, BF)])
+@pytest.mark.parametrize("lens,budget", [([900, 300, 301], 300), ([5000, 700, 90, 2000], 700), ([9000, 64, 2500], 2100), ([12000], 11990)])
+def test_evict_in_place_by_clusters(K, D, page, dtype, lens, budget):
+    """few rows of large budgets: two, four and eight CTAs move a row together"""
+    check_evict(K, lens, 2, D, page, dtype, budget, 4, 100, 34, True)
+
+
+def test_prefill_and_evict_on_side_streams_and_in_graphs(K):
+    """prefill whose pairs are cut along their keys, and evictions in place and to other pages, on three streams at once, each
+    with a workspace and results of its own; then captured, and the graphs replayed at once"""
+    g = gen(91)
+    qs, budget = 0.11, 700
+    calls, checks = [], []
+    for i, (n, m) in enumerate([(9000, 70), (12000, 33)]):
+        pool, bt, ln = R.make_cache([n, 300], 1, 128, 16, BF, g)
+        q = queries(m + 5, 4, 128, BF, g)
+        cu = torch.tensor([0, m, m + 5], dtype=torch.int32, device=DEV)
+        ws = K.Workspace(2, 1, 4, 128, bt.shape[1] * 16, DEV, new_tokens=m + 5)
+        out = torch.zeros(m + 5, 512, dtype=BF, device=DEV)
+        ref = []
+        for b, (s0, s1, L) in enumerate([(0, m, n), (m, m + 5, 300)]):
+            k, v = R.rows_of(pool, bt[b], L)
+            o, _, A, S = R.attend(q[s0:s1].double(), k, v, torch.arange(L - s1 + s0, L), qs, 0, 0)
+            ref.append((o, bound(o, A, S, 128, L, BF, True)))
+        o, tol = (torch.cat(x) for x in zip(*ref))
+        calls.append(lambda q=q, cu=cu, pool=pool, bt=bt, ln=ln, out=out, ws=ws: K.prefill(q, cu, pool, bt, ln, out, qs, ws=ws))
+        checks.append(lambda out=out, o=o, tol=tol, m=m: bool(((out.view(m + 5, 4, 128).double() - o).abs() <= tol).all()))
+    for in_place in (True, False):
+        lens = [3000, 650, 1200]
+        pool, bt, ln = R.make_cache(lens, 2, 128, 16, BF, g, poison=False)
+        start, w = pool.clone(), torch.rand(3, 2, bt.shape[1] * 16, generator=g).to(DEV)
+        dst = pool if in_place else torch.zeros(3 * 44, 2, 2, 16, 128, dtype=BF, device=DEV)
+        dbt = bt if in_place else torch.randperm(132, generator=g).int().view(3, 44).to(DEV)
+        kept, nl, nw = torch.empty(3, 2, budget, dtype=torch.int32, device=DEV), torch.empty(3, dtype=torch.int32, device=DEV), torch.empty(3, 2, budget, device=DEV)
+        exp, ref = (start if in_place else dst).clone(), [R.evict_ref(w[b], n, budget, 4, 64) for b, n in enumerate(lens)]
+        for b in range(3):
+            for h in range(2):
+                idx = torch.tensor(ref[b][h], device=DEV)
+                at = torch.arange(len(idx), device=DEV)
+                exp[dbt[b, at // 16].long(), h, :, at % 16] = start[bt[b, idx // 16].long(), h, :, idx % 16]
+        kw = {} if in_place else dict(dst_pool=dst, dst_table=dbt)
+
+        def call(pool=pool, bt=bt, ln=ln, w=w, kept=kept, nl=nl, nw=nw, kw=kw, start=start, dst=dst):
+            pool.copy_(start)
+            if kw:
+                dst.zero_()
+            K.evict(pool, bt, ln, w, budget, 4, 64, kept, nl, nw, **kw)
+
+        def check(dst=dst, exp=exp, kept=kept, nl=nl, ref=ref, lens=lens):
+            return torch.equal(dst, exp) and nl.tolist() == [min(n, budget) for n in lens] and \
+                all([x[:len(r)] for x, r in zip(kept[b].tolist(), ref[b])] == ref[b] for b in range(3) for r in ref[b])
+
+        calls.append(call)
+        checks.append(check)
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for c, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                c()
+    torch.cuda.synchronize()
+    assert all(c() for c in checks)
+    graphs = []
+    for c, s in zip(calls, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            c()
+    for _ in range(4):
+        for cg, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                cg.replay()
+    torch.cuda.synchronize()
+    assert all(c() for c in checks)
+
+
+def test_two_graphs_share_a_workspace_in_turn(K):
+    """a decode step and a prompt captured with the same workspace, replayed one after the other on one stream while the lengths
+    change under them"""
+    g = gen(92)
+    lens = [2000, 33, 700]
+    pool, bt, ln = R.make_cache(lens, 2, 128, 16, BF, g)
+    T, qs = 90, 0.1
+    ws = K.Workspace(3, 2, 4, 128, bt.shape[1] * 16, DEV, weights=True, new_tokens=T)
+    q1, qn = queries(3, 8, 128, BF, g), queries(T, 8, 128, BF, g)
+    cu = torch.tensor([0, 60, 60, T], dtype=torch.int32, device=DEV)
+    o1, on = torch.zeros(3, 1024, dtype=BF, device=DEV), torch.zeros(T, 1024, dtype=BF, device=DEV)
+    w = torch.zeros(3, 2, bt.shape[1] * 16, device=DEV)
+    steps = (lambda: K.attn(q1, pool, bt, ln, o1, ws, qs, weights=w)), (lambda: K.prefill(qn, cu, pool, bt, ln, on, qs, ws=ws))
+    graphs = []
+    for f in steps:
+        f()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            f()
+    for now in ([2000, 33, 700], [1, 0, 31], [1500, 20, 64]):
+        ln.copy_(torch.tensor(now, dtype=torch.int32))
+        for _ in range(3):
+            w.zero_()
+            for cg in graphs:
+                cg.replay()
+        check_attn(o1.view(3, 8, 128), q1, pool, bt, torch.tensor(now), qs, 0, 0, torch.zeros_like(w), w)
+        for b, (s0, s1) in enumerate([(0, 60), (60, 60), (60, T)]):
+            n, m = now[b], s1 - s0
+            lost = max(m - n, 0)
+            assert bool((on[s0:s0 + lost] == 0).all())
+            if m > lost:
+                k, v = R.rows_of(pool, bt[b], n)
+                o, _, A, S = R.attend(qn[s0 + lost:s1].double(), k, v, torch.arange(n - m + lost, n), qs, 0, 0)
+                assert bool(((on[s0 + lost:s1].view(-1, 8, 128).double() - o).abs() <= bound(o, A, S, 128, n, BF, True)).all())
+        assert int(ws.tickets.abs().max()) == 0
