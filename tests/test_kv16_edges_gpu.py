@@ -322,3 +322,53 @@ def test_two_graphs_share_a_workspace_in_turn(K):
                 o, _, A, S = R.attend(qn[s0 + lost:s1].double(), k, v, torch.arange(n - m + lost, n), qs, 0, 0)
                 assert bool(((on[s0 + lost:s1].view(-1, 8, 128).double() - o).abs() <= bound(o, A, S, 128, n, BF, True)).all())
         assert int(ws.tickets.abs().max()) == 0
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_that_follow_other_streams_wait_for_all_of_them(K, captured):
+    """rows written on two side streams, a copy on a third, and the attention that joins them by events: early launches wait for
+    every one of them, eagerly and as branches of a graph"""
+    g = gen(93)
+    B, Hkv, G, D, page, n = 8, 4, 4, 128, 16, 4000
+    width = -(-n // page)
+    pool = torch.zeros(B * width, Hkv, 2, page, D, dtype=BF, device=DEV)
+    bt = torch.randperm(B * width, generator=g).int().view(B, width).to(DEV)
+    t = torch.arange(n, device=DEV)
+    slots = (bt[:, t // page].long() * page + t % page).view(B, n)
+    kv = [torch.randn(B // 2 * n, 2 * Hkv, D, generator=g).to(BF).to(DEV) for _ in range(2)]
+    qs = [queries(B, Hkv * G, D, BF, g) for _ in range(2)]
+    q, ln, w = torch.empty_like(qs[0]), torch.zeros(B, dtype=torch.int32, device=DEV), torch.zeros(B, Hkv, width * page, device=DEV)
+    full = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    out = torch.zeros(B, Hkv * G * D, dtype=BF, device=DEV)
+    ws = K.Workspace(B, Hkv, G, D, width * page, DEV, weights=True)
+    sides = [torch.cuda.Stream() for _ in range(3)]
+
+    def step():
+        main = torch.cuda.current_stream()
+        pool.zero_(), ln.zero_(), w.zero_(), q.zero_()
+        for s in sides:
+            s.wait_stream(main)
+        for i in range(2):
+            with torch.cuda.stream(sides[i]):
+                K.write(kv[i], slots[i * B // 2:(i + 1) * B // 2].reshape(-1), pool)
+        with torch.cuda.stream(sides[2]):
+            q.copy_(qs[0])
+            ln.copy_(full)
+        for s in sides:
+            main.wait_stream(s)
+        K.attn(q, pool, bt, ln, out, ws, 0.1, weights=w)
+
+    step()
+    torch.cuda.synchronize()
+    check_attn(out.view(B, Hkv * G, D), qs[0], pool, bt, full, 0.1, 0, 0, torch.zeros_like(w), w)
+    first = out.clone(), w.clone()
+    run = step
+    if captured:
+        cg = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(cg):
+            step()
+        run = cg.replay
+    for _ in range(20):
+        run()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first[0]) and torch.equal(w, first[1])
