@@ -13,15 +13,18 @@
 // are, and a half that no query of the tile sees is left out.  The softmax reference is lazy: it moves when a row's
 // maximum has grown by more than 2^8, and only then is O rescaled.
 // Full waves of pairs run whole; the pairs of the last, partly filled wave are cut along their keys and joined where that is
-// shorter (4 x 512 over 32768: 1117 us with, 1163 without; the window case, whose pairs have 10 blocks: 418 with, 406 without).
+// shorter (4 x 512 over 32768: 1083 us with, 1182 without; prompts through a window, whose pairs have 10 blocks: 395 with, 394
+// without).
 //
 // V is taken as it lies (keys by dims): the second product's B operand is MN-major, K = keys.
 // P is rounded to the cache's type (2^-9 relative in bf16, 2^-12 in fp16: one rounding, like the output's own, which makes
-// the output's rms error up to sqrt 2 of its own rounding's); the row sums, S and O are 32-bit.
+// the output's rms error up to sqrt 2 of its own rounding's: 0.0022 of the output's rms in bf16 where its own rounding is
+// 0.0017); the row sums, S and O are 32-bit.
 //
-// Measured (bf16, D 128, G 4, page 16): 4 x 512 new tokens over 32768: 1.09 ms = 1.02 PFLOP/s under the power cap, where the
-// same pipeline without its softmax runs at 1.30 and cuBLAS at 1.40; prompts of 5544 to 7033 tokens through a window of 1024:
-// 0.395 ms = 0.75 PFLOP/s of visible pairs (1216 keys are computed for 1028 visible ones).  A step of 128 keys takes about
+// Measured (bf16, D 128, G 4, page 16): 4 x 512 new tokens over 32768: 1.08 to 1.12 ms = 0.99 to 1.02 PFLOP/s under the power cap,
+// where the same pipeline without its softmax runs at 1.30 and cuBLAS at 1.40; prompts of 5544 to 7033 tokens through a window of
+// 1024: 0.39 to 0.41 ms = 0.72 to 0.75 PFLOP/s of visible pairs (1216 keys are computed for 1028 visible ones; zeroing the values
+// that no query of a pair sees is 0.5 to 1 % of it, and nothing measurable of the other).  A step of 128 keys takes about
 // 3900 cycles, 2500 of them tensor (the N = 64 products of the halves cost 48 cycles instead of 32); the rest is latency of
 // the one softmax warp per tile and scheduler.  Measured and not kept: a polynomial 2^x for part of the weights (the MUFU is
 // half idle), two threads per row (104 registers a thread: spills), whole 128-key S tiles (the same time, windows 8 % slower),
@@ -165,8 +168,8 @@ FR_DEVI uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n
 FR_DEVI float4 f4(const uint32_t* v) {
   return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
 }
-// 16 dims of an output row times inv (zeros when !any); wide: rows are 32-byte aligned, a whole sector per store (the window case:
-// 418 us with, 435 without)
+// 16 dims of an output row times inv (zeros when !any); wide: rows are 32-byte aligned, a whole sector per store (prompts through
+// a window: 395 us with, 413 without; 4 x 512 over 32768, whose output is small: 1083 with, 1062 without)
 template <int DT> FR_DEVI void put16(uint16_t* out, float4 x, float4 y, float4 z, float4 t, float inv, bool any, bool wide) {
   uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (any) {

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(CT) k_write(const uint16_t* kv, long long kv_t
 cudaError_t write_rows(const uint16_t* kv, long long kv_ts, long long kv_hs, const long long* slots, int T, int Hkv, int D,
                        int page_sh, long long num_pages, uint16_t* pool, cudaStream_t st) {
   const long long n = static_cast<long long>(T) * 2 * Hkv * (D >> 3), nslots = num_pages << page_sh;
-  const int per = n > 148ll * 8 * 4 * CT ? 4 : 1;   // more than one piece for every thread the SMs hold: four in flight
+  const int per = n > 148ll * 8 * 4 * CT ? 4 : 1;   // more than four pieces for every thread the SMs hold: four in flight
                                                       // (65536 rows: 83 us, 111 one by one; 64 rows: the same)
   return launch(per == 4 ? k_write<4> : k_write<1>, static_cast<unsigned>((n + per * CT - 1) / (per * CT)), CT, 0, 0, st, kv, kv_ts, kv_hs,
                 slots, T, Hkv, D, page_sh, nslots, pool);

@@ -157,7 +157,7 @@ def write(kv, slots, pool):
 def attn(q, pool, block_table, seq_lens, out, ws, qscale, window=0, sinks=0, weights=None):
     """q [B, G Hkv, D] -> out [B, G Hkv D] (or [B, G Hkv, D]), rows 16-byte aligned; block_table int32 [B, width] (row stride 0
     allowed), seq_lens int32 [B]; qscale = softmax scale * log2(e).  Key j is seen when j < len and (window <= 0 or
-    j >= len - window or j < sinks); a row that sees no key gives zeros.  weights fp32 [B, Hkv, >= width * page] or None: the
+    j >= len - window or j < sinks); a row that sees no key, or only such with a score of -inf, gives zeros.  weights fp32 [B, Hkv, >= width * page] or None: the
     softmax weights of every seen key, summed over the G heads, are added to it."""
     npg, Hkv, page, D = _pool_ok(pool)
     B, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)
@@ -184,8 +184,9 @@ def prefill(q, cu_q, pool, block_table, seq_lens, out, qscale, window=0, sinks=0
     [B + 1]) and the last ones of its seq_lens[b] cached tokens (their keys and values are in the pages already).  The token
     at position p sees key j <= p when window <= 0 or j > p - window or j < sinks; one at a negative position gives zeros;
     rows of out that belong to no sequence are left as they are.  Cached rows that none of a sequence's new tokens sees may
-    hold anything (their pages may belong to others by now); the values of those that some see must be finite.  ws: a
-    Workspace made with new_tokens."""
+    hold anything (their pages may belong to others by now); the values of those that some see must be finite.  The softmax
+    weights are rounded to the pool's type before they meet the values (attn keeps them to 2^-17).  ws: a Workspace made with
+    new_tokens."""
     npg, Hkv, page, D = _pool_ok(pool)
     T, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)
     B = block_table.shape[0]

@@ -58,7 +58,8 @@ int k16_attn(int dtype, const void* q, long long q_bs, const void* pool, long lo
  * q [T, G*Hkv, D] (row stride q_ts), row b's tokens at [cu_q[b], cu_q[b + 1]) (int32 [B + 1], ascending, taken within
  * [0, T]); token i of n is at position p = len - n + i and sees key j <= p when (window <= 0 or j > p - window or j < sinks);
  * out [T, G*Hkv*D] (row stride o_ts).  A token that sees no key (p < 0) is written as zeros; rows of out that belong to no
- * sequence are left as they are.  Rows that none of the sequence's new tokens sees (behind the window of the first of them and
+ * sequence are left as they are.  The softmax weights meet the values in the pool's type (a rounding each, beside the output's
+ * own; sums are 32-bit), where k16_attn keeps them to 2^-17.  Rows that none of the sequence's new tokens sees (behind the window of the first of them and
  * not sinks) may hold anything, and their pages may belong to others by now; the values of rows that some of them see must be
  * finite (a weight of 0 times infinity is NaN: the sums run over whole blocks). */
 int k16_prefill(int dtype, const void* q, long long q_ts, int T, const int* cu_q, const void* pool, long long num_pages,
