@@ -188,8 +188,8 @@ int k16_evict(const void* pool, long long num_pages, const int* block_table, lon
   const long long count[3] = {groups * budget, B, groups * nw_len};
   for (int i = 0, j = 1; i < 3; ++i, j = (j + 1) % 3)
     if (meets(result[i], count[i], seq_lens, 1, B, B) || meets(result[i], count[i], weights, 1, w_span, w_span) ||
-        meets(result[i], count[i], block_table, B, bt_stride, bt_width) || meets(result[i], count[i], dst_table, B, dst_stride, dst_width) ||
-        meets(result[i], count[i], result[j], 1, count[j], count[j]))
+        meets(result[i], count[i], block_table, B, bt_stride, bt_width) ||
+        meets(result[i], count[i], dst_table, B, dst_stride, dst_width) || meets(result[i], count[i], result[j], 1, count[j], count[j]))
       return -3;
   a.c = make_cache(pool, num_pages, block_table, bt_stride, bt_width, seq_lens, Hkv, page);
   a.B = B;

@@ -157,8 +157,8 @@ def write(kv, slots, pool):
 def attn(q, pool, block_table, seq_lens, out, ws, qscale, window=0, sinks=0, weights=None):
     """q [B, G Hkv, D] -> out [B, G Hkv D] (or [B, G Hkv, D]), rows 16-byte aligned; block_table int32 [B, width] (row stride 0
     allowed), seq_lens int32 [B]; qscale = softmax scale * log2(e).  Key j is seen when j < len and (window <= 0 or
-    j >= len - window or j < sinks); a row that sees no key, or only such with a score of -inf, gives zeros.  weights fp32 [B, Hkv, >= width * page] or None: the
-    softmax weights of every seen key, summed over the G heads, are added to it."""
+    j >= len - window or j < sinks); a row that sees no key, or only such with a score of -inf, gives zeros.  weights fp32
+    [B, Hkv, >= width * page] or None: the softmax weights of every seen key, summed over the G heads, are added to it."""
     npg, Hkv, page, D = _pool_ok(pool)
     B, G, dt, qs, os_ = _q_ok(q, out, pool, Hkv, D)
     width, bs = _table_ok(block_table, B)
